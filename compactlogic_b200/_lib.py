@@ -19,6 +19,7 @@ W_LOGITS, W_PROBS, W_SELECT = 0, 1, 2
 _DTYPES = {torch.float32: CLB_F32, torch.float64: CLB_F64, torch.bfloat16: CLB_BF16, torch.float16: CLB_F16}
 
 _i64, _int, _p, _sz, _dbl = ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_double
+_u64 = ctypes.c_uint64
 
 # name -> (restype, argtypes)
 _SIGS = {
@@ -89,6 +90,16 @@ _SIGS = {
     "clb_packed_count_workspace_bytes": (_sz, [_i64, _i64, _i64]),
     "clb_packed_layer_count": (_int, [_p, _i64, _i64, _p, _p, _i64, _i64, _i64, _p, _i64, _i64, _p, _sz, _p]),
     "clb_packed_count": (_int, [_p, _i64, _i64, _i64, _i64, _p, _i64, _i64, _p]),
+    "clb_dropout": (_int, [_int, _p, _i64, _i64, _i64, _int, _dbl, _int, _u64, _u64, _p, _p, _i64, _p]),
+    "clb_dropout_advance": (_int, [_p, _p, _p]),
+    "clb_layer_norm_workspace_bytes": (_sz, [_int, _i64, _i64, _int, _int]),
+    "clb_layer_norm_forward": (_int, [_int, _p, _i64, _i64, _i64, _int, _p, _p, _dbl, _p, _i64, _p, _p, _p, _sz, _p]),
+    "clb_layer_norm_backward": (_int, [_int, _p, _i64, _p, _i64, _i64, _i64, _int, _p, _p, _p, _p, _i64, _p, _p, _p,
+                                       _sz, _p]),
+    "clb_action_logp": (_int, [_int, _p, _i64, _i64, _i64, _int, _p, _p, _dbl, _p, _p, _p]),
+    "clb_logit_grad": (_int, [_int, _p, _i64, _i64, _i64, _int, _p, _p, _dbl, _p, _p, _p, _p, _i64, _int, _p, _i64, _p]),
+    "clb_policy_loss": (_int, [_int, _p, _i64, _i64, _i64, _int, _p, _p, _p, _p, _p, _dbl, _dbl, _dbl, _dbl, _int, _p,
+                               _p, _p, _p, _p, _p, _p, _p, _p, _i64, _p]),
 }
 
 _lib = None

@@ -1,0 +1,397 @@
+"""Operators of a training step that stand before, between and after the logic layers, on hand-written sm_100a kernels:
+
+* ``layer_norm`` / ``LogicLayerNorm``: real-valued observations or activations, normalised over their features;
+* ``dropout`` / ``LogicDropout``: a mask from a counter-based generator, drawn again in the backward pass, never stored;
+* ``action_log_probs``: log-probability of one chosen class per row, differentiable;
+* ``policy_loss``: the clipped policy loss with a KL term, whose logit gradient is made in the same pass.
+
+All four take the layers' own storage (``[batch, features]`` views of feature-major memory) and ordinary row-major tensors
+alike, without copies, and run on the current stream.  A strided tensor that is neither is copied first.
+"""
+from typing import NamedTuple, Optional, Tuple, Union
+
+import torch
+
+from . import _lib as L
+from .functional import GradSlot, _incoming_grad, _outgoing_grad
+
+__all__ = ["LogicDropout", "LogicLayerNorm", "PolicyLoss", "action_log_probs", "dropout", "layer_norm", "policy_loss"]
+
+_LOW = (torch.bfloat16, torch.float16)
+
+
+# ------------------------------------------------------------------------------------------------------------ layouts
+def _matrix(x: torch.Tensor) -> Tuple[torch.Tensor, int, int]:
+    """A [n, d] tensor with one contiguous axis (a copy when ``x`` has none), whether that axis is n, and the other's
+    stride.  A tensor that is both (one row, one column) counts as rows."""
+    n, d = x.shape
+    sn, sd = x.stride()
+    if (sd == 1 or d <= 1) and (sn >= d or n <= 1):
+        return x, 0, sn if n > 1 else d
+    if (sn == 1 or n <= 1) and (sd >= n or d <= 1):
+        return x, 1, sd if d > 1 else n
+    return x.contiguous(), 0, d
+
+
+def _like(x: torch.Tensor, inner: int) -> torch.Tensor:
+    """A new dense [n, d] tensor with the contiguous axis of ``_matrix``."""
+    n, d = x.shape
+    return torch.empty_strided((n, d), (1, n) if inner else (d, 1), dtype=x.dtype, device=x.device)
+
+
+def _on_device(x: torch.Tensor, what: str, **others) -> None:
+    if not x.is_cuda:
+        raise RuntimeError("compactlogic_b200 kernels need CUDA tensors (there is no CPU fallback)")
+    for name, t in others.items():
+        if t is not None and t.device != x.device:
+            raise RuntimeError(f"{what}: {name} is on {t.device}, the input on {x.device}")
+
+
+# ------------------------------------------------------------------------------------------------------------ dropout
+def _drop(x: torch.Tensor, p: float, rescale: bool, seed: int, offset: int, rng: Optional[torch.Tensor]) -> torch.Tensor:
+    x, inner, ld = _matrix(x)
+    y = _like(x, inner)
+    n, d = x.shape
+    rows, cols = (d, n) if inner else (n, d)
+    L.call("clb_dropout", L.dtype_code(x.dtype), x.data_ptr(), ld, rows, cols, inner, p, rescale, seed, offset, L.ptr(rng),
+           y.data_ptr(), cols, L.stream(x.device))
+    return y
+
+
+class _DropoutFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, p, rescale, seed, offset, rng, in_slot, out_slot):
+        ctx.args = (p, rescale, seed, offset, rng)
+        ctx.in_slot, ctx.out_slot, ctx.dtype, ctx.shape = in_slot, out_slot, x.dtype, x.shape
+        return _drop(x, *ctx.args)
+
+    @staticmethod
+    def backward(ctx, gy):
+        slot = ctx.out_slot
+        if slot is not None and slot.grad is not None:
+            gy = _incoming_grad(gy.t(), slot, torch.float32).t()
+        gx = _drop(gy, *ctx.args)
+        if ctx.in_slot is not None:
+            ctx.in_slot.add(gx.float().t())
+            gx = torch.zeros((), dtype=ctx.dtype, device=gx.device).expand(ctx.shape)
+        return gx, None, None, None, None, None, None, None
+
+
+def _dropout(x, p, rescale, seed, offset, rng):
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"dropout: p must be in [0, 1], got {p}")
+    _on_device(x, "dropout", rng=rng)
+    L.dtype_code(x.dtype)
+    if x.dim() == 2:
+        # between logic layers with 16-bit activations the gradient is handed over in fp32, past autograd's rounding
+        out_slot = GradSlot() if x.dtype in _LOW and x.requires_grad and torch.is_grad_enabled() else None
+        y = _DropoutFn.apply(x, p, rescale, seed, offset, rng, getattr(x, "_clb_slot", None), out_slot)
+        if out_slot is not None:
+            y._clb_slot = out_slot
+        return y
+    flat = x.reshape(x.shape[0], -1) if x.dim() > 2 and x.shape[0] else x.reshape(1, -1)
+    return _DropoutFn.apply(flat, p, rescale, seed, offset, rng, None, None).reshape(x.shape)
+
+
+def dropout(x: torch.Tensor, p: float = 0.5, *, seed: int, offset: int = 0, rescale: bool = True) -> torch.Tensor:
+    """Zero each entry of ``x`` with probability ``p`` (in steps of 2^-32) and scale the others by 1 / (1 - p), or leave them
+    as they are with ``rescale=False`` (soft bits then stay in [0, 1]).
+
+    Entry (i, j) of ``x`` taken as [first axis, all others] is kept when its word of Philox4x32-10 under the key ``seed``
+    and the counter (j / 2, i / 2, ``offset``) is at least p 2^32: the mask depends on seed, offset and place alone, not
+    on layout, strides or type, and is not stored.  Use another ``offset`` for each pass.  A dropped entry is 0 whatever it
+    held."""
+    if not (0 <= seed < 1 << 64 and 0 <= offset < 1 << 64):
+        raise ValueError("dropout: seed and offset are unsigned 64-bit numbers")
+    return _dropout(x, p, rescale, seed, offset, None)
+
+
+class LogicDropout(torch.nn.Module):
+    """``dropout`` between logic layers, a new mask for each training pass; the identity in eval mode.
+
+    The buffer ``rng_state`` (int64 {seed, offset}) advances on the device, so a captured training step
+    (``compactlogic_b200.graph``) draws a new mask at each replay, and a loaded checkpoint continues the sequence.  ``seed``
+    defaults to a draw from torch's generator.  Passes of one module on several streams at once are not ordered."""
+
+    def __init__(self, p: float = 0.5, rescale: bool = True, seed: Optional[int] = None):
+        super().__init__()
+        if not 0.0 <= p <= 1.0:
+            raise ValueError(f"LogicDropout: p must be in [0, 1], got {p}")
+        if seed is None:
+            seed = int(torch.randint(0, 1 << 62, ()).item())
+        if not 0 <= seed < 1 << 63:
+            raise ValueError("LogicDropout: seed must be in [0, 2^63)")
+        self.p, self.rescale = float(p), bool(rescale)
+        self.register_buffer("rng_state", torch.tensor([seed, 0], dtype=torch.int64))
+
+    def forward(self, x):
+        if not self.training or self.p == 0.0:
+            return x
+        _on_device(x, "LogicDropout", rng_state=self.rng_state)
+        used = torch.empty(2, dtype=torch.int64, device=x.device)
+        L.call("clb_dropout_advance", L.ptr(self.rng_state), L.ptr(used), L.stream(x.device))
+        return _dropout(x, self.p, self.rescale, 0, 0, used)
+
+    def extra_repr(self):
+        return f"p={self.p}, rescale={self.rescale}"
+
+
+# --------------------------------------------------------------------------------------------------------- layer norm
+def _norm_forward(x, weight, bias, eps, keep):
+    """(y, x as laid out, its layout, mean, rstd); the last two None without ``keep``."""
+    x, inner, ld = _matrix(x)
+    n, d = x.shape
+    y = _like(x, inner)
+    code = L.dtype_code(x.dtype)
+    acc = L.acc_dtype(x.dtype)
+    mean, rstd = torch.empty((2, n), dtype=acc, device=x.device).unbind() if keep else (None, None)
+    nbytes = L.lib().clb_layer_norm_workspace_bytes(code, n, d, inner, 0)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+    L.call("clb_layer_norm_forward", code, x.data_ptr(), ld, n, d, inner, L.ptr(weight), L.ptr(bias), eps, y.data_ptr(),
+           n if inner else d, L.ptr(mean), L.ptr(rstd), L.ptr(ws), nbytes, L.stream(x.device))
+    return y, x, inner, mean, rstd
+
+
+class _LayerNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, x, ctx.inner, mean, rstd = _norm_forward(x, weight, bias, eps, True)
+        ctx.save_for_backward(x, weight, mean, rstd)
+        return y
+
+    @staticmethod
+    def backward(ctx, gy):
+        x, weight, mean, rstd = ctx.saved_tensors
+        n, d = x.shape
+        x, inner, ld = _matrix(x)
+        gy, g_inner, ldg = _matrix(gy)
+        if g_inner != inner and n > 1 and d > 1:
+            gy = gy.t().contiguous().t() if inner else gy.contiguous()
+        if inner:
+            ldg = gy.stride(1) if d > 1 else n
+        else:
+            ldg = gy.stride(0) if n > 1 else d
+        acc = L.acc_dtype(x.dtype)
+        gx = _like(x, inner) if ctx.needs_input_grad[0] else None
+        gw = torch.empty(d, dtype=acc, device=x.device) if ctx.needs_input_grad[1] else None
+        gb = torch.empty(d, dtype=acc, device=x.device) if ctx.needs_input_grad[2] else None
+        code = L.dtype_code(x.dtype)
+        nbytes = L.lib().clb_layer_norm_workspace_bytes(code, n, d, inner, 1)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+        L.call("clb_layer_norm_backward", code, x.data_ptr(), ld, gy.data_ptr(), ldg, n, d, inner, L.ptr(weight), L.ptr(mean),
+               L.ptr(rstd), L.ptr(gx), n if inner else d, L.ptr(gw), L.ptr(gb), L.ptr(ws), nbytes, L.stream(x.device))
+        return gx, gw, gb, None
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+               eps: float = 1e-5) -> torch.Tensor:
+    """(x - mean) / sqrt(var + eps) * weight + bias over the last axis (the features); the output has the layout of ``x``.
+
+    ``weight`` and ``bias`` (optional, [features]) are fp32 for fp32, bf16 and fp16 activations and fp64 for fp64, as the
+    layers' parameters are; statistics and the parameters' gradients are summed in that type, in a fixed order."""
+    _on_device(x, "layer_norm", weight=weight, bias=bias)
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise RuntimeError(f"layer_norm: expected [..., features], got shape {tuple(x.shape)}")
+    acc = L.acc_dtype(x.dtype)
+    L.dtype_code(x.dtype)
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None and (t.dtype != acc or t.shape != x.shape[-1:]):
+            raise RuntimeError(f"layer_norm: {name} must be {acc} [{x.shape[-1]}], got {t.dtype} {tuple(t.shape)}")
+    if not eps >= 0.0:
+        raise ValueError(f"layer_norm: eps must not be negative, got {eps}")
+    weight = weight if weight is None or weight.is_contiguous() else weight.contiguous()
+    bias = bias if bias is None or bias.is_contiguous() else bias.contiguous()
+    flat = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    if torch.is_grad_enabled() and (flat.requires_grad or (weight is not None and weight.requires_grad) or
+                                    (bias is not None and bias.requires_grad)):
+        y = _LayerNormFn.apply(flat, weight, bias, eps)
+    else:
+        y = _norm_forward(flat, weight, bias, eps, False)[0]
+    return y if x.dim() == 2 else y.reshape(x.shape)
+
+
+class LogicLayerNorm(torch.nn.Module):
+    """``layer_norm`` with learned fp32 weight and bias (``affine=False``: none)."""
+
+    def __init__(self, features: int, eps: float = 1e-5, affine: bool = True):
+        super().__init__()
+        self.features, self.eps = features, eps
+        self.weight = torch.nn.Parameter(torch.ones(features)) if affine else None
+        self.bias = torch.nn.Parameter(torch.zeros(features)) if affine else None
+
+    def forward(self, x):
+        if x.shape[-1:] != (self.features,):
+            raise RuntimeError(f"LogicLayerNorm({self.features}): got shape {tuple(x.shape)}")
+        w, b = self.weight, self.bias
+        if x.dtype == torch.float64 and w is not None:
+            w, b = w.double(), b.double()
+        return layer_norm(x, w, b, self.eps)
+
+    def extra_repr(self):
+        return f"{self.features}, eps={self.eps}, affine={self.weight is not None}"
+
+
+# ------------------------------------------------------------------------------------------------------------- losses
+def _rows_of(what, logits, actions, mask):
+    """Logits as [n, v] and the per-row arguments flattened to match."""
+    _on_device(logits, what, actions=actions, mask=mask)
+    L.dtype_code(logits.dtype)
+    lead = logits.shape[:-1]
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise RuntimeError(f"{what}: expected logits [..., classes], got shape {tuple(logits.shape)}")
+    if actions.shape != lead:
+        raise RuntimeError(f"{what}: actions must have shape {tuple(lead)}, got {tuple(actions.shape)}")
+    if actions.dtype != torch.int64:
+        if actions.is_floating_point() or actions.is_complex() or actions.dtype == torch.bool:
+            raise RuntimeError(f"{what}: actions must be integers, got {actions.dtype}")
+        actions = actions.long()
+    if mask is not None:
+        if mask.shape != lead or mask.dtype not in (torch.bool, torch.uint8):
+            raise RuntimeError(f"{what}: mask must be bool {tuple(lead)}, got {mask.dtype} {tuple(mask.shape)}")
+        mask = mask.reshape(-1).contiguous()
+    z = logits if logits.dim() == 2 else logits.reshape(-1, logits.shape[-1])
+    return z, actions.reshape(-1).contiguous(), mask, lead
+
+
+def _logit_grad(z, actions, mask, temperature, stats, slope, scale, upstream, up_stride, gz=None):
+    """gz for one upstream gradient; a given ``gz`` already holds the gradient for an upstream of 1."""
+    z, inner, ld = _matrix(z)
+    n, v = z.shape
+    fresh = gz is None
+    if fresh:
+        gz = _like(z, inner)
+    L.call("clb_logit_grad", L.dtype_code(z.dtype), z.data_ptr(), ld, n, v, inner, actions.data_ptr(), L.ptr(mask),
+           temperature, stats.data_ptr(), L.ptr(slope), L.ptr(scale), L.ptr(upstream), up_stride, not fresh, gz.data_ptr(),
+           n if inner else v, L.stream(z.device))
+    return gz
+
+
+def _logp_forward(z, actions, mask, temperature, keep):
+    z, inner, ld = _matrix(z)
+    n, v = z.shape
+    acc = L.acc_dtype(z.dtype)
+    logp = torch.empty(n, dtype=acc, device=z.device)
+    stats = torch.empty(2 * n, dtype=acc, device=z.device) if keep else None
+    L.call("clb_action_logp", L.dtype_code(z.dtype), z.data_ptr(), ld, n, v, inner, actions.data_ptr(), L.ptr(mask),
+           temperature, logp.data_ptr(), L.ptr(stats), L.stream(z.device))
+    return logp, z, stats
+
+
+class _LogProbFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, z, actions, mask, temperature):
+        logp, z, stats = _logp_forward(z, actions, mask, temperature, True)
+        ctx.save_for_backward(z, actions, mask, stats)
+        ctx.temperature = temperature
+        return logp
+
+    @staticmethod
+    def backward(ctx, g):
+        z, actions, mask, stats = ctx.saved_tensors
+        return _logit_grad(z, actions, mask, ctx.temperature, stats, None, None, g, g.stride(0)), None, None, None
+
+
+def _check_temperature(what, temperature):
+    if not temperature > 0.0:
+        raise ValueError(f"{what}: temperature must be positive, got {temperature}")
+
+
+def action_log_probs(logits: torch.Tensor, actions: torch.Tensor, *, mask: Optional[torch.Tensor] = None,
+                     temperature: float = 1.0) -> torch.Tensor:
+    """log softmax(logits / temperature)[..., actions], in the arithmetic type (fp32; fp64 for fp64 logits), differentiable
+    with respect to the logits.
+
+    ``logits`` [..., classes] in row-major or class-major storage (as GroupSum returns it), ``actions`` integers [...].
+    Rows where ``mask`` (bool [...]) is False are not read: their value and gradient are 0 and their action may be
+    anything.  In other rows an action outside [0, classes) gives NaN."""
+    z, act, m, lead = _rows_of("action_log_probs", logits, actions, mask)
+    _check_temperature("action_log_probs", temperature)
+    if z.requires_grad and torch.is_grad_enabled():
+        logp = _LogProbFn.apply(z, act, m, temperature)
+    else:
+        logp = _logp_forward(z, act, m, temperature, False)[0]
+    return logp if len(lead) == 1 else logp.reshape(lead)
+
+
+class PolicyLoss(NamedTuple):
+    """What ``policy_loss`` returns: the loss (differentiable), and per row, without gradients, the chosen actions'
+    log-probabilities, the ratios to the old policy, and the KL term (None without ``ref_log_probs``)."""
+    loss: torch.Tensor
+    log_probs: torch.Tensor
+    ratio: torch.Tensor
+    kl: Optional[torch.Tensor]
+
+
+class _PolicyLossFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, z, actions, mask, adv, old, ref, low, high, kl_coef, temperature, reduction, grad):
+        z, inner, ld = _matrix(z)
+        n, v = z.shape
+        acc = L.acc_dtype(z.dtype)
+        dev = z.device
+        logp, ratio, row_loss = (torch.empty(n, dtype=acc, device=dev) for _ in range(3))
+        kl = torch.empty(n, dtype=acc, device=dev) if ref is not None else None
+        slope, stats = torch.empty(3 * n, dtype=acc, device=dev).split((n, 2 * n)) if grad else (None, None)
+        loss, scale = torch.empty((), dtype=acc, device=dev), torch.empty((), dtype=acc, device=dev)
+        # the mean's and the sum's gradient is made in the same pass, for an upstream gradient of 1
+        gz = _like(z, inner) if grad and reduction != "none" else None
+        L.call("clb_policy_loss", L.dtype_code(z.dtype), z.data_ptr(), ld, n, v, inner, actions.data_ptr(), L.ptr(mask),
+               adv.data_ptr(), old.data_ptr(), L.ptr(ref), low, high, kl_coef, temperature, reduction == "mean",
+               loss.data_ptr(), scale.data_ptr(), row_loss.data_ptr(), logp.data_ptr(), ratio.data_ptr(), L.ptr(kl),
+               L.ptr(slope), L.ptr(stats), L.ptr(gz), n if inner else v, L.stream(dev))
+        if grad:
+            ctx.save_for_backward(z, actions, mask, slope, stats, scale)
+            ctx.gz, ctx.temperature = gz, temperature
+            ctx.per_row = reduction == "none"
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(*(t for t in (logp, ratio, kl) if t is not None))
+        return row_loss if reduction == "none" else loss, logp, ratio, kl
+
+    @staticmethod
+    def backward(ctx, g, *unused):
+        if g is None:
+            return (None,) * 12
+        z, actions, mask, slope, stats, scale = ctx.saved_tensors
+        # The gradient made in the forward pass is handed out once; a later call (a retained graph) makes another.
+        gz, ctx.gz = ctx.gz, None
+        gz = _logit_grad(z, actions, mask, ctx.temperature, stats, slope, scale, g, g.stride(0) if ctx.per_row else 0, gz)
+        return (gz,) + (None,) * 11
+
+
+def policy_loss(logits: torch.Tensor, actions: torch.Tensor, advantages: torch.Tensor, old_log_probs: torch.Tensor, *,
+                ref_log_probs: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None,
+                clip: Union[float, Tuple[float, float]] = 0.2, kl_coef: float = 0.0, temperature: float = 1.0,
+                reduction: str = "mean") -> PolicyLoss:
+    """The clipped policy loss with a KL term, over the rows where ``mask`` is True (all without a mask):
+
+        lp = action_log_probs(logits, actions, temperature),  ratio = exp(lp - old_log_probs)
+        row = -min(ratio * advantages, clamp(ratio, 1 - clip_low, 1 + clip_high) * advantages) + kl_coef * kl
+        kl = exp(ref_log_probs - lp) - (ref_log_probs - lp) - 1
+
+    ``reduction``: "mean" over the counted rows (0 when none counts), "sum", or "none" (per row).  ``clip`` is one bound or
+    (clip_low, clip_high).  The gradient goes to ``logits`` alone; the other arguments are data.  Rows that do not count
+    are not read, give zeros, and get a zero gradient; a counted row whose action is outside [0, classes) gives NaN.
+
+    With "mean" and "sum" the logit gradient is computed in the forward pass, for an upstream gradient of 1; ``backward``
+    hands it over, or computes it anew where the upstream gradient is another (a scaled loss)."""
+    z, act, m, lead = _rows_of("policy_loss", logits, actions, mask)
+    _check_temperature("policy_loss", temperature)
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError(f"policy_loss: reduction must be mean, sum or none, got {reduction!r}")
+    low, high = clip if isinstance(clip, (tuple, list)) else (clip, clip)
+    if not (low >= 0.0 and high >= 0.0):
+        raise ValueError(f"policy_loss: clip must not be negative, got {clip}")
+    acc = L.acc_dtype(z.dtype)
+    given = []
+    for name, t in (("advantages", advantages), ("old_log_probs", old_log_probs), ("ref_log_probs", ref_log_probs)):
+        if t is not None:
+            _on_device(z, "policy_loss", **{name: t})
+            if t.shape != lead:
+                raise RuntimeError(f"policy_loss: {name} must have shape {tuple(lead)}, got {tuple(t.shape)}")
+            t = t.detach().to(acc).reshape(-1).contiguous()
+        given.append(t)
+    out = _PolicyLossFn.apply(z, act, m, *given, low, high, kl_coef, temperature, reduction,
+                              z.requires_grad and torch.is_grad_enabled())
+    if len(lead) != 1:
+        out = tuple(t if t is None or (i == 0 and reduction != "none") else t.reshape(lead) for i, t in enumerate(out))
+    return PolicyLoss(*out)

@@ -23,6 +23,8 @@
  *      same tensor layouts, argument meaning and results.
  *   2. clb_logic_* / clb_slots_* / clb_packed_* are the native fast path used by the Python layers
  *      (softmax and its backward fused, int32 slot tables, fused GroupSum, bit-packed inference).
+ *   3. clb_dropout* / clb_layer_norm_* / clb_action_logp / clb_policy_loss / clb_logit_grad are the operators of a
+ *      training step that stand before, between and after the layers; the reference leaves these to PyTorch.
  */
 #ifndef COMPACTLOGIC_B200_H
 #define COMPACTLOGIC_B200_H
@@ -410,6 +412,64 @@ int clb_packed_layer_count(const uint64_t* x, int64_t ldx, int64_t nwords, const
 /* Packed GroupSum over stored words [rows, nwords] uint64: same accumulation as above. */
 int clb_packed_count(const uint64_t* words, int64_t rows, int64_t nwords, int64_t k, int64_t class_size,
                      int32_t* counts, int64_t sample0, int64_t nsamples, clb_stream_t stream);
+
+/* ======================= 3. operators of a training step around the layers =======================
+ * No reference counterpart.  Activations and logits are [n, d] (n samples or tokens) of any enum clb_dtype, in one of two
+ * storages: rows (element (i, j) at i * ld + j) or, with batch_inner / feature_major / class_major != 0, the layers' own
+ * (element (i, j) at j * ld + i).  Parameters, statistics, losses and per-row values are of the arithmetic type (fp32, or
+ * fp64 for fp64 activations).  Sums are deterministic: a call repeated on the same inputs gives the same bits.
+ */
+
+/* y = keep ? x * s : 0 with s = 1 / (1 - p) when rescale, else 1.  keep(i, j) = word >= round(p 2^32), word =
+ * Philox4x32-10(counter = (j / 2, i / 2, offset low, offset high), key = (seed low, seed high))[2 (i % 2) + (j % 2)], i the
+ * sample and j the feature: the mask depends on nothing else and is not stored.  The gradient is the same call on grad_y.
+ * rows / cols are the sizes of the strided and the contiguous axis, at most 2^33 each; batch_inner != 0 says that the
+ * contiguous one is the samples.  rng (optional): device int64 {seed, offset} read in place of the two arguments. */
+int clb_dropout(int dtype, const void* x, int64_t ldx, int64_t rows, int64_t cols, int batch_inner, double p, int rescale,
+                uint64_t seed, uint64_t offset, const int64_t* rng, void* y, int64_t ldy, clb_stream_t stream);
+
+/* used[0..1] = state[0..1] = {seed, offset}; state[1] += 1: the generator of one pass and the step to the next, on the
+ * device, so that a captured graph draws a new mask at each replay. */
+int clb_dropout_advance(int64_t* state, int64_t* used, clb_stream_t stream);
+
+/* Layer norm over the d features: y = (x - mean) * rstd * weight + bias, rstd = 1 / sqrt(var + eps), weight and bias
+ * optional.  mean / rstd [n] (optional in the forward pass) are what the backward pass needs.  Backward: gx, gw, gb each
+ * optional; gw and gb [d] are written (zero for n = 0).  `workspace`: clb_layer_norm_workspace_bytes() bytes, 256-byte
+ * aligned (null where that is 0). */
+size_t clb_layer_norm_workspace_bytes(int dtype, int64_t n, int64_t d, int feature_major, int backward);
+int clb_layer_norm_forward(int dtype, const void* x, int64_t ldx, int64_t n, int64_t d, int feature_major,
+                           const void* weight, const void* bias, double eps, void* y, int64_t ldy, void* mean, void* rstd,
+                           void* workspace, size_t workspace_bytes, clb_stream_t stream);
+int clb_layer_norm_backward(int dtype, const void* x, int64_t ldx, const void* gy, int64_t ldgy, int64_t n, int64_t d,
+                            int feature_major, const void* weight, const void* mean, const void* rstd, void* gx,
+                            int64_t ldgx, void* gw, void* gb, void* workspace, size_t workspace_bytes,
+                            clb_stream_t stream);
+
+/* logp[i] = z[i, a_i] / T - log sum_j exp(z[i, j] / T) over v classes.  mask (optional, uint8 [n]): rows with 0 are not
+ * read and give 0; in the others an action outside [0, v) gives NaN.  stats (optional, [2, n]): each row's maximum and
+ * sum, for clb_logit_grad. */
+int clb_action_logp(int dtype, const void* z, int64_t ldz, int64_t n, int64_t v, int class_major, const int64_t* actions,
+                    const uint8_t* mask, double temperature, void* logp, void* stats, clb_stream_t stream);
+
+/* gz[i, j] = c_i / T ([j = a_i] - softmax(z[i] / T)_j), c_i = slope[i] * scale[0] * upstream[i * upstream_stride]; each of
+ * the three may be null (1).  Rows with mask 0 get zeros.  unless_one: do nothing when the scalar upstream[0] is 1 (gz
+ * then already holds that gradient).  T as in the call that made stats. */
+int clb_logit_grad(int dtype, const void* z, int64_t ldz, int64_t n, int64_t v, int class_major, const int64_t* actions,
+                   const uint8_t* mask, double temperature, const void* stats, const void* slope, const void* scale,
+                   const void* upstream, int64_t upstream_stride, int unless_one, void* gz, int64_t ldgz,
+                   clb_stream_t stream);
+
+/* Clipped policy loss with a KL term.  Per counted row (mask != 0, or all), with lp as in clb_action_logp:
+ *   ratio = exp(lp - old_logp),  q = ref_logp - lp,  kl = exp(q) - q - 1  (no KL term with ref_logp == NULL)
+ *   row_loss = -min(ratio A, clip(ratio, 1 - clip_low, 1 + clip_high) A) + kl_coef kl
+ * loss[0] (optional) = scale * sum of row_loss, scale[0] = 1 / max(1, counted rows) with mean, else 1.  Rows that do not
+ * count give 0 in logp, ratio, kl and row_loss.  slope [n] = d row_loss / d lp and stats [2, n] are what clb_logit_grad
+ * needs.  gz (optional): the gradient of the loss with respect to z, for an upstream gradient of 1 (needs slope, stats). */
+int clb_policy_loss(int dtype, const void* z, int64_t ldz, int64_t n, int64_t v, int class_major, const int64_t* actions,
+                    const uint8_t* mask, const void* advantages, const void* old_logp, const void* ref_logp,
+                    double clip_low, double clip_high, double kl_coef, double temperature, int mean, void* loss,
+                    void* scale, void* row_loss, void* logp, void* ratio, void* kl, void* slope, void* stats, void* gz,
+                    int64_t ldgz, clb_stream_t stream);
 
 #ifdef __cplusplus
 }
