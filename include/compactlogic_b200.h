@@ -423,7 +423,7 @@ int clb_packed_count(const uint64_t* words, int64_t rows, int64_t nwords, int64_
 /* y = keep ? x * s : 0 with s = 1 / (1 - p) when rescale, else 1.  keep(i, j) = word >= round(p 2^32), word =
  * Philox4x32-10(counter = (j / 2, i / 2, offset low, offset high), key = (seed low, seed high))[2 (i % 2) + (j % 2)], i the
  * sample and j the feature: the mask depends on nothing else and is not stored.  The gradient is the same call on grad_y.
- * rows / cols are the sizes of the strided and the contiguous axis, at most 2^33 each; batch_inner != 0 says that the
+ * rows / cols are the sizes of the strided and the contiguous axis, at most 2^32 each; batch_inner != 0 says that the
  * contiguous one is the samples.  rng (optional): device int64 {seed, offset} read in place of the two arguments. */
 int clb_dropout(int dtype, const void* x, int64_t ldx, int64_t rows, int64_t cols, int batch_inner, double p, int rescale,
                 uint64_t seed, uint64_t offset, const int64_t* rng, void* y, int64_t ldy, clb_stream_t stream);

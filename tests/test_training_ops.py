@@ -49,7 +49,7 @@ def test_c_entry_points_refuse_without_a_gpu():
     assert lib.clb_dropout(9, 16, 4, 4, 4, 0, 0.5, 1, 0, 0, None, 16, 4, None) == L.CLB_ERR_DTYPE
     assert lib.clb_dropout(0, None, 4, 4, 4, 0, 0.5, 1, 0, 0, None, 16, 4, None) == L.CLB_ERR_INVALID
     assert lib.clb_dropout(0, 16, 4, -1, 4, 0, 0.5, 1, 0, 0, None, 16, 4, None) == L.CLB_ERR_INVALID
-    assert lib.clb_dropout(0, 16, 4, 4, (1 << 33) + 1, 0, 0.5, 1, 0, 0, None, 16, 4, None) == L.CLB_ERR_INVALID
+    assert lib.clb_dropout(0, 16, 4, 4, (1 << 32) + 1, 0, 0.5, 1, 0, 0, None, 16, 4, None) == L.CLB_ERR_INVALID
     assert lib.clb_dropout(0, None, 0, 0, 4, 0, 0.5, 1, 0, 0, None, None, 0, None) == L.CLB_OK  # nothing to do
     assert lib.clb_dropout_advance(None, 16, None) == L.CLB_ERR_INVALID
     norm = [0, 16, 8, 4, 8, 0, None, None, 1e-5, 16, 8, None, None, None, 0, None]
