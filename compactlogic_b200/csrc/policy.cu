@@ -12,6 +12,7 @@
 
 #include "common.cuh"
 #include "kernels.h"
+#include "vec.cuh"
 
 namespace clb {
 
@@ -40,18 +41,24 @@ template <typename A> struct RowArgs {
     const A *adv, *old_lp, *ref;
     A lo, hi, beta;
     A *ratio, *kl, *slope, *row_loss;
+    // the gradient of the same pass (null `gz` of the kernels: none): gz[i * gn + j * gv], scaled by `fixed` or scale[0]
+    int64_t gn, gv;
+    const A* scale;
+    A fixed;
 };
 
-// One row from its maximum and sum; returns d loss_i / d lp_i before the scale.
+// One row from its maximum and sum; returns d loss_i / d lp_i before the scale.  write: put the results down.
 template <typename T, typename A = typename Acc<T>::type>
-__device__ A finish_row(const T* __restrict__ z, const RowArgs<A>& a, int64_t i, A m, A s) {
+__device__ A finish_row(const T* __restrict__ z, const RowArgs<A>& a, int64_t i, A m, A s, bool write = true) {
     const int64_t act = a.actions[i];
     A lp = (A)NAN;
     if (act >= 0 && act < a.v) lp = (to_acc(z[i * a.sn + act * a.sv]) - m) * a.inv_t - log(s);
-    a.logp[i] = lp;
-    if (a.stats != nullptr) {
-        a.stats[i] = m;
-        a.stats[a.n + i] = s;
+    if (write) {
+        a.logp[i] = lp;
+        if (a.stats != nullptr) {
+            a.stats[i] = m;
+            a.stats[a.n + i] = s;
+        }
     }
     if (a.adv == nullptr) return (A)0;
     const A adv = a.adv[i], r = exp(lp - a.old_lp[i]);
@@ -59,15 +66,19 @@ __device__ A finish_row(const T* __restrict__ z, const RowArgs<A>& a, int64_t i,
     const A free_ = r * adv, kept = held * adv;
     A loss = -(free_ <= kept ? free_ : kept), slope = free_ <= kept ? -free_ : (A)0;
     if (free_ != free_) loss = slope = free_;
-    a.ratio[i] = r;
+    A kl = 0;
     if (a.ref != nullptr) {
         const A q = a.ref[i] - lp, e = expm1(q);
-        a.kl[i] = e - q;
-        loss += a.beta * (e - q);
+        kl = e - q;
+        loss += a.beta * kl;
         slope -= a.beta * e;
     }
-    a.row_loss[i] = loss;
-    if (a.slope != nullptr) a.slope[i] = slope;
+    if (write) {
+        a.ratio[i] = r;
+        if (a.ref != nullptr) a.kl[i] = kl;
+        a.row_loss[i] = loss;
+        if (a.slope != nullptr) a.slope[i] = slope;
+    }
     return slope;
 }
 
@@ -110,18 +121,247 @@ template <typename A> __device__ __forceinline__ void warp_merge(Run<A>& r, A fa
     }
 }
 
-// Logits contiguous: one block per row, which reads its row once.
+// What a row's gradient needs beside its logits: gz_j = c [j = act] + w exp((z_j - m) / T) with w = -c / s.
+template <typename A> struct RowGrad { A m, c, w; };
+
+template <typename A> __device__ __forceinline__ RowGrad<A> row_grad(const RowArgs<A>& a, A slope, A m, A s) {
+    // in the order of the gradient kernels below, which then give the same bits for an upstream gradient of 1
+    const A c = slope * (a.scale != nullptr ? a.scale[0] : a.fixed) * a.inv_t;
+    return {m, c, -c / s};
+}
+
+// Rows contiguous, held in registers as 16-byte windows: window k of row i has the entries VEC k - shift ..., where `shift`
+// is how far the row starts past a 16-byte boundary.  Entries outside the row read as -inf and are not written.
+template <typename T, int NV> struct RowPart {
+    static constexpr int VEC = 16 / sizeof(T);
+    Pack<T, VEC> x[NV];
+
+    // windows first, first + stride, ... of the row at `row`
+    __device__ __forceinline__ void load(const T* __restrict__ row, int shift, int64_t v, int64_t first, int stride) {
+#pragma unroll
+        for (int u = 0; u < NV; ++u) {
+            const int64_t c = VEC * (first + (int64_t)u * stride) - shift;
+            if (c >= 0 && c + VEC <= v) {
+                x[u].load(row + c);
+            } else {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) x[u].raw(j, c + j >= 0 && c + j < v ? row[c + j] : T(-INFINITY));
+            }
+        }
+    }
+    __device__ __forceinline__ void sum(Run<float>& r, float factor) const {
+        float f[VEC];
+        float m = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < NV; ++u) {
+            x[u].get(f);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) m = fmaxf(m, f[j]);  // a NaN is left to the sum
+        }
+        r.m = m;
+        const float safe = m == -INFINITY ? 0.f : m;
+        float s[4] = {};
+        if (fabsf(safe) < 1e37f) {  // the product with the factor stays finite: one multiply-add an element
+            const float mk = safe * factor;
+#pragma unroll
+            for (int u = 0; u < NV; ++u) {
+                x[u].get(f);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) s[j & 3] += soft_exp(fmaf(f[j], factor, -mk));
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < NV; ++u) {
+                x[u].get(f);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) s[j & 3] += soft_exp((f[j] - safe) * factor);
+            }
+        }
+        r.s = (s[0] + s[1]) + (s[2] + s[3]);
+    }
+    // the row's gradient without the chosen action's own term; `same`: out's windows lie as the row's
+    __device__ __forceinline__ void grad(T* __restrict__ out, int shift, bool same, int64_t v, int64_t first, int stride,
+                                         const RowGrad<float>& g, float factor) const {
+        const bool tame = fabsf(g.m) < 1e37f;
+        const float mk = g.m * factor;
+#pragma unroll
+        for (int u = 0; u < NV; ++u) {
+            const int64_t c = VEC * (first + (int64_t)u * stride) - shift;
+            if (c + VEC <= 0 || c >= v) continue;
+            float f[VEC];
+            x[u].get(f);
+            if (tame) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) f[j] = g.w * soft_exp(fmaf(f[j], factor, -mk));
+            } else {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) f[j] = g.w * soft_exp((f[j] - g.m) * factor);
+            }
+            Pack<T, VEC> y;
+            y.put(f);
+            if (same && c >= 0 && c + VEC <= v) {
+                y.store(out + c);
+            } else {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j)
+                    if (c + j >= 0 && c + j < v) out[c + j] = y.raw(j);
+            }
+        }
+    }
+    __device__ __forceinline__ static void zero(T* __restrict__ out, int shift, bool same, int64_t v, int64_t first,
+                                                int stride) {
+#pragma unroll
+        for (int u = 0; u < NV; ++u) {
+            const int64_t c = VEC * (first + (int64_t)u * stride) - shift;
+            if (same && c >= 0 && c + VEC <= v) {
+                Pack<T, VEC> y = {};
+                y.store(out + c);
+            } else {
+                for (int j = 0; j < VEC; ++j)
+                    if (c + j >= 0 && c + j < v) out[c + j] = T(0.f);
+            }
+        }
+    }
+};
+
+template <typename T> __device__ __forceinline__ int shift_of(const T* p) {
+    return (int)((reinterpret_cast<uintptr_t>(p) / sizeof(T)) % (16 / sizeof(T)));
+}
+
+// The chosen action's own entry, written by the thread that wrote its window before.
 template <typename T>
-__global__ void __launch_bounds__(256) rows_forward_kernel(const T* __restrict__ z, RowArgs<typename Acc<T>::type> a) {
+__device__ __forceinline__ void put_action(T* out, const T* row, int64_t act, const RowGrad<float>& g, float factor) {
+    const float z = to_acc(row[act]);
+    out[act] = from_acc<T>(g.c + g.w * soft_exp((z - g.m) * factor));
+}
+
+// Short rows: G lanes of a warp per row, the row's windows in their registers.
+template <typename T, int NV, int G>
+__global__ void __launch_bounds__(128) rows_group_kernel(const T* __restrict__ z, T* __restrict__ gz, RowArgs<float> a) {
+    const int lane = threadIdx.x % G;
+    const int64_t i = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / G;
+    const bool in = i < a.n, live = in && (a.mask == nullptr || a.mask[i]);
+    const T* row = z + (in ? i : 0) * a.sn;
+    const int shift = shift_of(row);
+    RowPart<T, NV> part;
+    Run<float> r;
+    if (live) {
+        part.load(row, shift, a.v, lane, G);
+        part.sum(r, a.factor);
+    }
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1) {
+        const float m2 = __shfl_xor_sync(0xffffffffu, r.m, o), s2 = __shfl_xor_sync(0xffffffffu, r.s, o);
+        r.merge(m2, s2, a.factor);
+    }
+    float slope = 0.f;
+    if (lane == 0 && in) {
+        if (live)
+            slope = finish_row<T>(z, a, i, r.m, r.s);
+        else
+            skip_row(a, i);
+    }
+    if (gz == nullptr) return;
+    slope = __shfl_sync(0xffffffffu, slope, 0, G);
+    if (!in) return;
+    T* out = gz + i * a.gn;
+    const bool same = shift_of(out) == shift;
+    if (!live) {
+        RowPart<T, NV>::zero(out, shift, same, a.v, lane, G);
+        return;
+    }
+    const RowGrad<float> g = row_grad(a, slope, r.m, r.s);
+    part.grad(out, shift, same, a.v, lane, G, g, a.factor);
+    const int64_t act = a.actions[i];
+    if (act >= 0 && act < a.v && (act + shift) / RowPart<T, NV>::VEC % G == lane) put_action(out, row, act, g, a.factor);
+}
+
+// Longer rows: a cluster of `parts` blocks per row (one block for parts = 1), NV windows a thread.  The blocks give each
+// other their warps' maxima and sums through distributed shared memory, and every block finishes the row by itself.
+template <typename T, int NV>
+__global__ void __launch_bounds__(512, 2) rows_block_kernel(const T* __restrict__ z, T* __restrict__ gz, RowArgs<float> a,
+                                                            int parts) {
+    constexpr int VEC = RowPart<T, NV>::VEC;
+    __shared__ float2 runs[8 * 16];
+    __shared__ RowGrad<float> shared;
+    const int64_t i = blockIdx.x / (unsigned)parts;
+    const int rank = (int)(blockIdx.x % (unsigned)parts), warps = blockDim.x >> 5, warp = threadIdx.x >> 5,
+              lane = threadIdx.x & 31;
+    const T* row = z + i * a.sn;
+    const int shift = shift_of(row);
+    const int64_t first = (int64_t)rank * blockDim.x * NV + threadIdx.x;
+    T* out = gz != nullptr ? gz + i * a.gn : nullptr;
+    const bool same = gz != nullptr && shift_of(out) == shift;
+    if (a.mask != nullptr && !a.mask[i]) {  // the same in every block of the cluster
+        if (rank == 0 && threadIdx.x == 0) skip_row(a, i);
+        if (gz != nullptr) RowPart<T, NV>::zero(out, shift, same, a.v, first, blockDim.x);
+        return;
+    }
+    if (parts > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // this block has started
+    RowPart<T, NV> part;
+    part.load(row, shift, a.v, first, blockDim.x);
+    Run<float> r;
+    part.sum(r, a.factor);
+    warp_merge(r, a.factor);
+    if (parts > 1) {
+        asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+        if (lane < parts) {
+            uint32_t local = (uint32_t)__cvta_generic_to_shared(&runs[rank * warps + warp]), remote;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(lane));
+            asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(remote), "f"(r.m), "f"(r.s) : "memory");
+        }
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    } else {
+        if (lane == 0) runs[warp] = make_float2(r.m, r.s);
+        __syncthreads();
+    }
+    if (warp == 0) {
+        Run<float> t;
+        for (int k = lane; k < parts * warps; k += 32) t.merge(runs[k].x, runs[k].y, a.factor);
+        warp_merge(t, a.factor);
+        if (lane == 0) {
+            const float slope = finish_row<T>(z, a, i, t.m, t.s, rank == 0);
+            if (gz != nullptr) shared = row_grad(a, slope, t.m, t.s);
+        }
+    }
+    if (gz == nullptr) return;
+    __syncthreads();
+    const RowGrad<float> g = shared;
+    part.grad(out, shift, same, a.v, first, blockDim.x, g, a.factor);
+    const int64_t act = a.actions[i];
+    if (act >= 0 && act < a.v) {
+        const int64_t k = (act + shift) / VEC - (int64_t)rank * blockDim.x * NV;
+        if (k >= 0 && k < (int64_t)blockDim.x * NV && k % blockDim.x == threadIdx.x) put_action(out, row, act, g, a.factor);
+    }
+}
+
+// Any row length, any type: one block per row, which reads its row once for the sum and once more for the gradient.
+template <typename T>
+__global__ void __launch_bounds__(512) rows_stream_kernel(const T* __restrict__ z, T* __restrict__ gz,
+                                                          RowArgs<typename Acc<T>::type> a) {
     using A = typename Acc<T>::type;
-    __shared__ A sm[8], ss[8];
+    __shared__ A sm[16], ss[16];
+    __shared__ RowGrad<A> shared;
     for (int64_t i = blockIdx.x; i < a.n; i += gridDim.x) {
+        const T* row = z + i * a.sn;
+        T* out = gz != nullptr ? gz + i * a.gn : nullptr;
         if (a.mask != nullptr && !a.mask[i]) {
             if (threadIdx.x == 0) skip_row(a, i);
+            if (gz != nullptr)
+                for (int64_t j = threadIdx.x; j < a.v; j += blockDim.x) out[j] = T(0.f);
             continue;
         }
         Run<A> r;
-        for (int64_t j = threadIdx.x; j < a.v; j += blockDim.x) r.add(to_acc(z[i * a.sn + j * a.sv]), a.factor);
+        int64_t j = threadIdx.x;
+        for (; j + 7 * blockDim.x < a.v; j += 8 * blockDim.x) {
+            A f[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) f[u] = to_acc(row[j + u * blockDim.x]);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) r.add(f[u], a.factor);
+        }
+        for (; j < a.v; j += blockDim.x) r.add(to_acc(row[j]), a.factor);
         warp_merge(r, a.factor);
         __syncthreads();
         if ((threadIdx.x & 31) == 0) {
@@ -131,31 +371,118 @@ __global__ void __launch_bounds__(256) rows_forward_kernel(const T* __restrict__
         __syncthreads();
         if (threadIdx.x == 0) {
             for (int w = 1; w < (int)(blockDim.x >> 5); ++w) r.merge(sm[w], ss[w], a.factor);
-            finish_row<T>(z, a, i, r.m, r.s);
+            const A slope = finish_row<T>(z, a, i, r.m, r.s);
+            if (gz != nullptr) shared = row_grad(a, slope, r.m, r.s);
+        }
+        if (gz == nullptr) continue;
+        __syncthreads();
+        const RowGrad<A> g = shared;
+        const int64_t act = a.actions[i];
+        const bool tame = sizeof(A) == 4 && fabs(g.m) < (A)1e37;  // as RowPart::grad, bit for bit
+        const A mk = g.m * a.factor;
+        for (j = threadIdx.x; j < a.v; j += blockDim.x) {
+            const A f = to_acc(row[j]);
+            const A e = g.w * soft_exp(tame && j != act ? fma(f, a.factor, -mk) : (f - g.m) * a.factor);
+            out[j] = from_acc<T>(j == act ? g.c + e : e);
         }
     }
 }
 
-// Samples contiguous: 32 x 8 threads per 32 rows, the lanes along the rows.
-template <typename T>
-__global__ void __launch_bounds__(256) cols_forward_kernel(const T* __restrict__ z, RowArgs<typename Acc<T>::type> a) {
+constexpr int kMostWarps = 64, kHeld = 16;  // warps of a cluster along the classes, classes a thread holds
+
+// Samples contiguous: 32 rows a block, the lanes along them, blockDim.y warps (and `parts` blocks of a cluster) along the
+// classes.  HELD: each thread's classes fit its registers, else the logits are read again for the gradient.
+template <typename T, bool HELD>
+__global__ void __launch_bounds__(512) cols_kernel(const T* __restrict__ z, T* __restrict__ gz,
+                                                   RowArgs<typename Acc<T>::type> a, int parts) {
     using A = typename Acc<T>::type;
-    __shared__ A sm[8][33], ss[8][33];
-    const int64_t i = (int64_t)blockIdx.x * 32 + threadIdx.x;
-    const bool live = i < a.n && (a.mask == nullptr || a.mask[i]);
+    constexpr int R = kHeld;
+    __shared__ A sm[kMostWarps][32], ss[kMostWarps][32];
+    __shared__ RowGrad<A> shared[32];
+    const int64_t i = (int64_t)(blockIdx.x / (unsigned)parts) * 32 + threadIdx.x;
+    const int rank = (int)(blockIdx.x % (unsigned)parts), warps = blockDim.y, stride = parts * warps;
+    const int64_t first = rank * warps + threadIdx.y;
+    const bool in = i < a.n, live = in && (a.mask == nullptr || a.mask[i]);
+    const T* row = z + (in ? i : 0);
+    if (parts > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     Run<A> r;
-    if (live)
-        for (int64_t j = threadIdx.y; j < a.v; j += blockDim.y) r.add(to_acc(z[i * a.sn + j * a.sv]), a.factor);
-    sm[threadIdx.y][threadIdx.x] = r.m;
-    ss[threadIdx.y][threadIdx.x] = r.s;
+    A f[R];
+    if (live) {
+        for (int64_t j = first; j < a.v; j += (int64_t)R * stride) {
+#pragma unroll
+            for (int u = 0; u < R; ++u) f[u] = j + u * stride < a.v ? to_acc(row[(j + u * stride) * a.sv]) : lowest<A>();
+            A top = lowest<A>();
+#pragma unroll
+            for (int u = 0; u < R; ++u) top = f[u] > top ? f[u] : top;
+            if (top > r.m) {
+                r.s *= soft_exp((r.m - top) * a.factor);
+                r.m = top;
+            }
+            const A safe = r.m == lowest<A>() ? (A)0 : r.m;
+#pragma unroll
+            for (int u = 0; u < R; ++u)
+                if (j + u * stride < a.v) r.s += soft_exp((f[u] - safe) * a.factor);
+            if (HELD) break;
+        }
+    }
+    if (parts > 1) {
+        asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+        for (int p = 0; p < parts; ++p) {
+            uint32_t at[2] = {(uint32_t)__cvta_generic_to_shared(&sm[first][threadIdx.x]),
+                              (uint32_t)__cvta_generic_to_shared(&ss[first][threadIdx.x])};
+            const A val[2] = {r.m, r.s};
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                uint32_t remote;
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(at[k]), "r"(p));
+                if constexpr (sizeof(A) == 4)
+                    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote), "f"((float)val[k]) : "memory");
+                else
+                    asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(remote), "d"((double)val[k]) : "memory");
+            }
+        }
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    } else if (warps > 1) {
+        sm[first][threadIdx.x] = r.m;
+        ss[first][threadIdx.x] = r.s;
+        __syncthreads();
+    }
+    if (threadIdx.y == 0 && in) {
+        if (live) {
+            if (stride > 1) {
+                r = Run<A>();
+                for (int w = 0; w < stride; ++w) r.merge(sm[w][threadIdx.x], ss[w][threadIdx.x], a.factor);
+            }
+            const A slope = finish_row<T>(z, a, i, r.m, r.s, rank == 0);
+            if (gz != nullptr) shared[threadIdx.x] = row_grad(a, slope, r.m, r.s);
+        } else if (rank == 0) {
+            skip_row(a, i);
+        }
+    }
+    if (gz == nullptr) return;
     __syncthreads();
-    if (threadIdx.y != 0 || i >= a.n) return;
+    if (!in) return;
+    T* out = gz + i;
     if (!live) {
-        skip_row(a, i);
+        for (int64_t j = first; j < a.v; j += stride) out[j * a.gv] = T(0.f);
         return;
     }
-    for (int w = 1; w < (int)blockDim.y; ++w) r.merge(sm[w][threadIdx.x], ss[w][threadIdx.x], a.factor);
-    finish_row<T>(z, a, i, r.m, r.s);
+    const RowGrad<A> g = shared[threadIdx.x];
+    const int64_t act = a.actions[i];
+    for (int64_t j = first; j < a.v; j += (int64_t)R * stride) {
+        if (!HELD) {
+#pragma unroll
+            for (int u = 0; u < R; ++u) f[u] = j + u * stride < a.v ? to_acc(row[(j + u * stride) * a.sv]) : (A)0;
+        }
+#pragma unroll
+        for (int u = 0; u < R; ++u)
+            if (j + u * stride < a.v) {
+                const A e = g.w * soft_exp((f[u] - g.m) * a.factor);
+                out[(j + u * stride) * a.gv] = from_acc<T>(j + u * stride == act ? g.c + e : e);
+            }
+        if (HELD) break;
+    }
 }
 
 template <typename A> struct GradArgs {
@@ -182,80 +509,187 @@ __global__ void __launch_bounds__(256) logit_grad_kernel(const T* __restrict__ z
         const int64_t i = COLS ? b * 32 + threadIdx.x : b;
         if (i >= a.n) continue;
         const bool live = a.mask == nullptr || a.mask[i];
-        A c = 0, m = 0, inv = 0;
+        A c = 0, m = 0, w = 0;
         int64_t act = -1;
         if (live) {
             c = (a.slope != nullptr ? a.slope[i] : (A)1) * scale * (a.upstream != nullptr ? a.upstream[i * a.up_stride] : (A)1) *
                 a.inv_t;
             m = a.stats[i];
-            inv = (A)1 / a.stats[a.n + i];
             act = a.actions[i];
             if (act < 0 || act >= a.v) c = (A)NAN;
+            w = -c / a.stats[a.n + i];
         }
         for (int64_t j = COLS ? threadIdx.y : threadIdx.x; j < a.v; j += COLS ? blockDim.y : blockDim.x) {
             A g = 0;
             if (live) {
-                g = -c * (soft_exp((to_acc(z[i * a.sn + j * a.sv]) - m) * a.factor) * inv);
-                if (j == act) g += c;
+                g = w * soft_exp((to_acc(z[i * a.sn + j * a.sv]) - m) * a.factor);
+                if (j == act) g = c + g;
             }
             gz[i * a.gn + j * a.gv] = from_acc<T>(g);
         }
     }
 }
 
-// Counted rows, and the loss from the rows' losses: one block, a fixed order of summation.
-template <typename A>
-__global__ void __launch_bounds__(1024) loss_kernel(const A* __restrict__ row_loss, const uint8_t* __restrict__ mask,
-                                                    int64_t n, int mean, A* loss, A* scale) {
-    __shared__ A sh[32];
-    __shared__ long long sc[32];
-    A s = 0;
-    long long c = 0;
-    for (int64_t i = threadIdx.x; i < n; i += blockDim.x) {
-        s += row_loss[i];
-        c += mask == nullptr || mask[i];
+// The same for contiguous rows, in 16-byte windows: blockDim.y rows a block, `chunks` blocks along a row.
+template <typename T, int NV>
+__global__ void __launch_bounds__(256) rows_grad_kernel(const T* __restrict__ z, T* __restrict__ gz, GradArgs<float> a,
+                                                        unsigned chunks) {
+    if (a.unless_one && a.upstream[0] == 1.f) return;
+    const int64_t i = (int64_t)(blockIdx.x / chunks) * blockDim.y + threadIdx.y;
+    if (i >= a.n) return;
+    const T* row = z + i * a.sn;
+    T* out = gz + i * a.gn;
+    const int shift = shift_of(row);
+    const bool same = shift_of(out) == shift;
+    const int64_t first = (int64_t)(blockIdx.x % chunks) * blockDim.x * NV + threadIdx.x;
+    if (a.mask != nullptr && !a.mask[i]) {
+        RowPart<T, NV>::zero(out, shift, same, a.v, first, blockDim.x);
+        return;
     }
-    s = warp_sum(s);
+    RowPart<T, NV> part;
+    part.load(row, shift, a.v, first, blockDim.x);
+    const int64_t act = a.actions[i];
+    float c = (a.slope != nullptr ? a.slope[i] : 1.f) * (a.scale != nullptr ? a.scale[0] : 1.f) *
+              (a.upstream != nullptr ? a.upstream[i * a.up_stride] : 1.f) * a.inv_t;
+    if (act < 0 || act >= a.v) c = NAN;
+    const RowGrad<float> g = {a.stats[i], c, -c / a.stats[a.n + i]};
+    part.grad(out, shift, same, a.v, first, blockDim.x, g, a.factor);
+    if (act >= 0 && act < a.v) {
+        const int64_t k = (act + shift) / RowPart<T, NV>::VEC - (int64_t)(blockIdx.x % chunks) * blockDim.x * NV;
+        if (k >= 0 && k < (int64_t)blockDim.x * NV && k % blockDim.x == threadIdx.x) put_action(out, row, act, g, a.factor);
+    }
+}
+
+// scale = 1 / (number of counted rows): one block.
+template <typename A>
+__global__ void __launch_bounds__(1024) count_kernel(const uint8_t* __restrict__ mask, int64_t n, A* scale) {
+    __shared__ int64_t sc[32];
+    int64_t c = 0;
+    const int64_t head = (16 - (reinterpret_cast<uintptr_t>(mask) & 15)) & 15;
+    const int64_t vecs = n > head ? (n - head) / 16 : 0;
+    for (int64_t k = threadIdx.x; k < vecs; k += blockDim.x) {
+        const uint4 v = *reinterpret_cast<const uint4*>(mask + head + 16 * k);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) c += __popc(__vcmpne4(w[q], 0)) / 8;
+    }
+    // the up to 15 entries before the first vector and after the last
+    const int64_t done = 16 * vecs, rest = n - done;
+    if (threadIdx.x < rest) c += mask[threadIdx.x < head ? threadIdx.x : threadIdx.x + done] != 0;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
-    if ((threadIdx.x & 31) == 0) {
-        sh[threadIdx.x >> 5] = s;
-        sc[threadIdx.x >> 5] = c;
-    }
+    if ((threadIdx.x & 31) == 0) sc[threadIdx.x >> 5] = c;
     __syncthreads();
     if (threadIdx.x >= 32) return;
-    s = warp_sum(sh[threadIdx.x]);
-    c = sc[threadIdx.x];
+    c = threadIdx.x < (blockDim.x >> 5) ? sc[threadIdx.x] : 0;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
+    if (threadIdx.x == 0) scale[0] = (A)1 / (A)(c > 0 ? c : 1);
+}
+
+// loss = scale * sum of the rows' losses: one block, a fixed order of summation.  `fixed` (when >= 0) is the scale where no
+// count was needed, and is put down for the backward pass.
+template <typename A>
+__global__ void __launch_bounds__(1024) loss_kernel(const A* __restrict__ row_loss, int64_t n, A fixed, A* loss, A* scale) {
+    __shared__ A sh[32];
+    A s[4] = {};
+    int64_t i = threadIdx.x;
+    for (; i + 3 * blockDim.x < n; i += 4 * blockDim.x) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) s[u] += row_loss[i + u * blockDim.x];
+    }
+    for (; i < n; i += blockDim.x) s[0] += row_loss[i];
+    A t = warp_sum((s[0] + s[1]) + (s[2] + s[3]));
+    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = t;
+    __syncthreads();
+    if (threadIdx.x >= 32) return;
+    t = warp_sum(threadIdx.x < (blockDim.x >> 5) ? sh[threadIdx.x] : (A)0);
     if (threadIdx.x == 0) {
-        const A f = mean ? (A)1 / (A)(c > 0 ? c : 1) : (A)1;
-        scale[0] = f;
-        if (loss != nullptr) loss[0] = s * f;
+        if (fixed >= 0) scale[0] = fixed;
+        if (loss != nullptr) loss[0] = t * (fixed >= 0 ? fixed : scale[0]);
     }
 }
 
 unsigned blocks(int64_t n) { return (unsigned)(n < (1 << 30) ? n : (1 << 30)); }
 
+template <typename P> struct Same { using type = P; };  // a parameter that is not deduced
+
 template <typename T> struct Logits {
     using A = typename Acc<T>::type;
 
-    static cudaError_t forward(const void* z, const RowArgs<A>& a, bool cols, cudaStream_t s) {
-        if (cols)
-            cols_forward_kernel<T><<<blocks(ceil_div64(a.n, 32)), dim3(32, 8), 0, s>>>((const T*)z, a);
-        else
-            rows_forward_kernel<T><<<blocks(a.n), 256, 0, s>>>((const T*)z, a);
+    // gz null: no gradient
+    static cudaError_t forward(const void* z, void* gz, const RowArgs<A>& a, bool cols, cudaStream_t s) {
         count_launches(1);
-        return cudaGetLastError();
+        return cols ? forward_cols((const T*)z, (T*)gz, a, s) : forward_rows((const T*)z, (T*)gz, a, s);
+    }
+
+    template <typename... P> static cudaError_t launch(void (*kernel)(P...), int64_t grid, dim3 block, int parts, cudaStream_t s,
+                                                       typename Same<P>::type... args) {
+        if (grid > 0x7FFFFFFF) return cudaErrorInvalidValue;
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3((unsigned)grid);
+        cfg.blockDim = block;
+        cfg.stream = s;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = (unsigned)parts;
+        at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = parts > 1 ? 1 : 0;
+        return cudaLaunchKernelEx(&cfg, kernel, args...);
+    }
+
+    static cudaError_t forward_cols(const T* z, T* gz, const RowArgs<A>& a, cudaStream_t s) {
+        // warps along the classes until each thread holds its classes, over up to four blocks of a cluster
+        const int64_t need = ceil_div64(a.v, kHeld);
+        const int parts = need <= 16 ? 1 : need <= 32 ? 2 : 4;
+        const int warps = need < 16 ? (int)need : kMostWarps / 4;
+        const int64_t grid = ceil_div64(a.n, 32) * parts;
+        return a.v <= (int64_t)kHeld * warps * parts
+                   ? launch(cols_kernel<T, true>, grid, dim3(32, warps), parts, s, z, gz, a, parts)
+                   : launch(cols_kernel<T, false>, grid, dim3(32, warps), parts, s, z, gz, a, parts);
+    }
+
+    static cudaError_t forward_rows(const T* z, T* gz, const RowArgs<A>& a, cudaStream_t s) {
+        if constexpr (sizeof(A) == 4) {
+            constexpr int VEC = 16 / sizeof(T);
+            // the most windows that a row takes, whatever its shift
+            const bool aligned = reinterpret_cast<uintptr_t>(z) % 16 == 0 && (a.n == 1 || a.sn % VEC == 0);
+            const int64_t w = ceil_div64(a.v + (aligned ? 0 : VEC - 1), VEC);
+            auto group = [&](auto kernel, int g) { return launch(kernel, ceil_div64(a.n * g, 128), dim3(128), 1, s, z, gz, a); };
+            if (w <= 4) return group(rows_group_kernel<T, 1, 4>, 4);
+            if (w <= 16) return group(rows_group_kernel<T, 1, 16>, 16);
+            if (w <= 32) return group(rows_group_kernel<T, 1, 32>, 32);
+            if (w <= 64) return group(rows_group_kernel<T, 2, 32>, 32);
+            if (w <= 128) return group(rows_group_kernel<T, 4, 32>, 32);
+            auto threads = [](int64_t k) { return dim3((unsigned)(ceil_div64(k, 32) * 32)); };
+            if (w <= 4 * 512) return launch(rows_block_kernel<T, 4>, a.n, threads(ceil_div64(w, 4)), 1, s, z, gz, a, 1);
+            for (int parts = 1; parts <= 8; parts *= 2)
+                if (w <= (int64_t)parts * 8 * 512)
+                    return launch(rows_block_kernel<T, 8>, a.n * parts, threads(ceil_div64(w, 8 * parts)), parts, s, z, gz, a,
+                                  parts);
+        }
+        return launch(rows_stream_kernel<T>, a.n, dim3(512), 1, s, z, gz, a);
     }
 
     static cudaError_t backward(const void* z, void* gz, const GradArgs<A>& a, bool cols, cudaStream_t s) {
-        if (cols)
-            logit_grad_kernel<T, true><<<blocks(ceil_div64(a.n, 32)), dim3(32, 8), 0, s>>>((const T*)z, (T*)gz, a);
-        else
-            logit_grad_kernel<T, false><<<blocks(a.n), 256, 0, s>>>((const T*)z, (T*)gz, a);
         count_launches(1);
-        return cudaGetLastError();
+        if (cols) {
+            logit_grad_kernel<T, true><<<blocks(ceil_div64(a.n, 32)), dim3(32, 8), 0, s>>>((const T*)z, (T*)gz, a);
+            return cudaGetLastError();
+        }
+        if constexpr (sizeof(A) == 4) {
+            constexpr int NV = 4;
+            const int64_t w = ceil_div64(a.v + 16 / sizeof(T) - 1, 16 / sizeof(T));
+            unsigned bx = 4;
+            while (bx < 256 && bx * NV < w) bx *= 2;
+            const int64_t chunks = ceil_div64(w, bx * NV);
+            return launch(rows_grad_kernel<T, NV>, ceil_div64(a.n, 256 / bx) * chunks, dim3(bx, 256 / bx), 1, s, (const T*)z,
+                          (T*)gz, a, (unsigned)chunks);
+        } else {
+            logit_grad_kernel<T, false><<<blocks(a.n), 256, 0, s>>>((const T*)z, (T*)gz, a);
+            return cudaGetLastError();
+        }
     }
 
     static int logp(const void* z, int64_t ldz, int64_t n, int64_t v, bool cols, const int64_t* actions,
@@ -264,7 +698,7 @@ template <typename T> struct Logits {
         fill(a, ldz, n, v, cols, actions, mask, t);
         a.logp = (A*)logp;
         a.stats = (A*)stats;
-        return status(forward(z, a, cols, s));
+        return status(forward(z, nullptr, a, cols, s));
     }
 
     static void fill(RowArgs<A>& a, int64_t ldz, int64_t n, int64_t v, bool cols, const int64_t* actions,
@@ -322,13 +756,21 @@ template <typename T> struct Logits {
         a.kl = (A*)kl;
         a.slope = (A*)slope;
         a.row_loss = (A*)row_loss;
+        a.gn = cols ? 1 : ldgz;
+        a.gv = cols ? ldgz : 1;
+        const bool count = mean && mask != nullptr;  // else the scale is known here
+        a.fixed = mean ? (A)1 / (A)(n > 0 ? n : 1) : (A)1;
+        if (count) {
+            a.scale = (const A*)scale;
+            count_kernel<A><<<1, 1024, 0, s>>>(mask, n, (A*)scale);
+            count_launches(1);
+            if (const int st = status(cudaGetLastError())) return st;
+        }
         if (n > 0)
-            if (const int st = status(forward(z, a, cols, s))) return st;
-        loss_kernel<A><<<1, 1024, 0, s>>>((const A*)row_loss, mask, n, mean, (A*)loss, (A*)scale);
+            if (const int st = status(forward(z, gz, a, cols, s))) return st;
+        loss_kernel<A><<<1, 1024, 0, s>>>((const A*)row_loss, n, count ? (A)-1 : a.fixed, (A*)loss, (A*)scale);
         count_launches(1);
-        if (const int st = status(cudaGetLastError())) return st;
-        if (gz == nullptr || n == 0) return CLB_OK;
-        return grad(z, ldz, n, v, cols, actions, mask, t, stats, slope, scale, nullptr, 0, 0, gz, ldgz, s);
+        return status(cudaGetLastError());
     }
 };
 
