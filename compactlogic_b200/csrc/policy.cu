@@ -130,37 +130,61 @@ template <typename A> __device__ __forceinline__ RowGrad<A> row_grad(const RowAr
     return {m, c, -c / s};
 }
 
+template <typename T> struct Two;  // a pair of 16-bit elements as the packed maximum takes it
+template <> struct Two<__nv_bfloat16> {
+    using type = __nv_bfloat162;
+    static __device__ __forceinline__ type of(uint32_t w) { return *reinterpret_cast<const type*>(&w); }
+};
+template <> struct Two<__half> {
+    using type = __half2;
+    static __device__ __forceinline__ type of(uint32_t w) { return *reinterpret_cast<const type*>(&w); }
+};
+
 // Rows contiguous, held in registers as 16-byte windows: window k of row i has the entries VEC k - shift ..., where `shift`
-// is how far the row starts past a 16-byte boundary.  Entries outside the row read as -inf and are not written.
+// is how far the row starts past a 16-byte boundary.  Entries outside the row read as -inf and are not written.  A row held
+// this way is short enough for 32-bit indexes.
 template <typename T, int NV> struct RowPart {
     static constexpr int VEC = 16 / sizeof(T);
     Pack<T, VEC> x[NV];
 
     // windows first, first + stride, ... of the row at `row`
-    __device__ __forceinline__ void load(const T* __restrict__ row, int shift, int64_t v, int64_t first, int stride) {
+    __device__ __forceinline__ void load(const T* __restrict__ row, int shift, int v, int first, int stride) {
+        const unsigned whole = v >= VEC ? v - VEC + 1 : 0;  // windows that start in [0, whole) lie in the row
+        int c = VEC * first - shift;
 #pragma unroll
-        for (int u = 0; u < NV; ++u) {
-            const int64_t c = VEC * (first + (int64_t)u * stride) - shift;
-            if (c >= 0 && c + VEC <= v) {
+        for (int u = 0; u < NV; ++u, c += VEC * stride) {
+            if ((unsigned)c < whole) {
                 x[u].load(row + c);
             } else {
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) x[u].raw(j, c + j >= 0 && c + j < v ? row[c + j] : T(-INFINITY));
+                for (int j = 0; j < VEC; ++j) x[u].raw(j, (unsigned)(c + j) < (unsigned)v ? row[c + j] : T(-INFINITY));
             }
         }
     }
-    __device__ __forceinline__ void sum(Run<float>& r, float factor) const {
-        float f[VEC];
-        float m = -INFINITY;
+    // the largest entry, a NaN left aside (the sum meets it)
+    __device__ __forceinline__ float top() const {
+        if constexpr (sizeof(T) == 2) {
+            typename Two<T>::type m[2] = {Two<T>::of(x[0].w[0]), Two<T>::of(x[0].w[1])};
 #pragma unroll
-        for (int u = 0; u < NV; ++u) {
-            x[u].get(f);
+            for (int u = 0; u < NV; ++u)
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) m = fmaxf(m, f[j]);  // a NaN is left to the sum
+                for (int k = 0; k < 4; ++k) m[k & 1] = __hmax2(m[k & 1], Two<T>::of(x[u].w[k]));
+            m[0] = __hmax2(m[0], m[1]);
+            return fmaxf(to_acc(m[0].x), to_acc(m[0].y));
+        } else {
+            float m[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int u = 0; u < NV; ++u)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) m[j & 1] = fmaxf(m[j & 1], x[u].raw(j));
+            return fmaxf(m[0], m[1]);
         }
+    }
+    __device__ __forceinline__ void sum(Run<float>& r, float factor) const {
+        const float m = fmaxf(top(), -INFINITY);  // NaN where all entries are
         r.m = m;
         const float safe = m == -INFINITY ? 0.f : m;
-        float s[4] = {};
+        float f[VEC], s[4] = {};
         if (fabsf(safe) < 1e37f) {  // the product with the factor stays finite: one multiply-add an element
             const float mk = safe * factor;
 #pragma unroll
@@ -180,14 +204,15 @@ template <typename T, int NV> struct RowPart {
         r.s = (s[0] + s[1]) + (s[2] + s[3]);
     }
     // the row's gradient without the chosen action's own term; `same`: out's windows lie as the row's
-    __device__ __forceinline__ void grad(T* __restrict__ out, int shift, bool same, int64_t v, int64_t first, int stride,
+    __device__ __forceinline__ void grad(T* __restrict__ out, int shift, bool same, int v, int first, int stride,
                                          const RowGrad<float>& g, float factor) const {
         const bool tame = fabsf(g.m) < 1e37f;
         const float mk = g.m * factor;
+        const unsigned whole = same && v >= VEC ? v - VEC + 1 : 0;
+        int c = VEC * first - shift;
 #pragma unroll
-        for (int u = 0; u < NV; ++u) {
-            const int64_t c = VEC * (first + (int64_t)u * stride) - shift;
-            if (c + VEC <= 0 || c >= v) continue;
+        for (int u = 0; u < NV; ++u, c += VEC * stride) {
+            if (c >= v) break;
             float f[VEC];
             x[u].get(f);
             if (tame) {
@@ -199,28 +224,22 @@ template <typename T, int NV> struct RowPart {
             }
             Pack<T, VEC> y;
             y.put(f);
-            if (same && c >= 0 && c + VEC <= v) {
-                y.store(out + c);
-            } else {
-#pragma unroll
-                for (int j = 0; j < VEC; ++j)
-                    if (c + j >= 0 && c + j < v) out[c + j] = y.raw(j);
-            }
+            put(out, c, whole, v, y);
         }
     }
-    __device__ __forceinline__ static void zero(T* __restrict__ out, int shift, bool same, int64_t v, int64_t first,
-                                                int stride) {
+    __device__ __forceinline__ static void put(T* __restrict__ out, int c, unsigned whole, int v, const Pack<T, VEC>& y) {
+        if ((unsigned)c < whole) {
+            y.store(out + c);
+        } else {
 #pragma unroll
-        for (int u = 0; u < NV; ++u) {
-            const int64_t c = VEC * (first + (int64_t)u * stride) - shift;
-            if (same && c >= 0 && c + VEC <= v) {
-                Pack<T, VEC> y = {};
-                y.store(out + c);
-            } else {
-                for (int j = 0; j < VEC; ++j)
-                    if (c + j >= 0 && c + j < v) out[c + j] = T(0.f);
-            }
+            for (int j = 0; j < VEC; ++j)
+                if ((unsigned)(c + j) < (unsigned)v) out[c + j] = y.raw(j);
         }
+    }
+    __device__ __forceinline__ static void zero(T* __restrict__ out, int shift, bool same, int v, int first, int stride) {
+        const unsigned whole = same && v >= VEC ? v - VEC + 1 : 0;
+        const Pack<T, VEC> y = {};
+        for (int u = 0, c = VEC * first - shift; u < NV; ++u, c += VEC * stride) put(out, c, whole, v, y);
     }
 };
 
@@ -238,7 +257,7 @@ __device__ __forceinline__ void put_action(T* out, const T* row, int64_t act, co
 // Short rows: G lanes of a warp per row, the row's windows in their registers.
 template <typename T, int NV, int G>
 __global__ void __launch_bounds__(128) rows_group_kernel(const T* __restrict__ z, T* __restrict__ gz, RowArgs<float> a) {
-    const int lane = threadIdx.x % G;
+    const int lane = threadIdx.x % G, v = (int)a.v;
     const int64_t i = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / G;
     const bool in = i < a.n, live = in && (a.mask == nullptr || a.mask[i]);
     const T* row = z + (in ? i : 0) * a.sn;
@@ -246,7 +265,7 @@ __global__ void __launch_bounds__(128) rows_group_kernel(const T* __restrict__ z
     RowPart<T, NV> part;
     Run<float> r;
     if (live) {
-        part.load(row, shift, a.v, lane, G);
+        part.load(row, shift, v, lane, G);
         part.sum(r, a.factor);
     }
 #pragma unroll
@@ -267,13 +286,13 @@ __global__ void __launch_bounds__(128) rows_group_kernel(const T* __restrict__ z
     T* out = gz + i * a.gn;
     const bool same = shift_of(out) == shift;
     if (!live) {
-        RowPart<T, NV>::zero(out, shift, same, a.v, lane, G);
+        RowPart<T, NV>::zero(out, shift, same, v, lane, G);
         return;
     }
     const RowGrad<float> g = row_grad(a, slope, r.m, r.s);
-    part.grad(out, shift, same, a.v, lane, G, g, a.factor);
+    part.grad(out, shift, same, v, lane, G, g, a.factor);
     const int64_t act = a.actions[i];
-    if (act >= 0 && act < a.v && (act + shift) / RowPart<T, NV>::VEC % G == lane) put_action(out, row, act, g, a.factor);
+    if (act >= 0 && act < v && ((int)act + shift) / RowPart<T, NV>::VEC % G == lane) put_action(out, row, act, g, a.factor);
 }
 
 // Longer rows: a cluster of `parts` blocks per row (one block for parts = 1), NV windows a thread.  The blocks give each
@@ -289,17 +308,17 @@ __global__ void __launch_bounds__(512, 2) rows_block_kernel(const T* __restrict_
               lane = threadIdx.x & 31;
     const T* row = z + i * a.sn;
     const int shift = shift_of(row);
-    const int64_t first = (int64_t)rank * blockDim.x * NV + threadIdx.x;
+    const int first = rank * blockDim.x * NV + threadIdx.x, v = (int)a.v;
     T* out = gz != nullptr ? gz + i * a.gn : nullptr;
     const bool same = gz != nullptr && shift_of(out) == shift;
     if (a.mask != nullptr && !a.mask[i]) {  // the same in every block of the cluster
         if (rank == 0 && threadIdx.x == 0) skip_row(a, i);
-        if (gz != nullptr) RowPart<T, NV>::zero(out, shift, same, a.v, first, blockDim.x);
+        if (gz != nullptr) RowPart<T, NV>::zero(out, shift, same, v, first, blockDim.x);
         return;
     }
     if (parts > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // this block has started
     RowPart<T, NV> part;
-    part.load(row, shift, a.v, first, blockDim.x);
+    part.load(row, shift, v, first, blockDim.x);
     Run<float> r;
     part.sum(r, a.factor);
     warp_merge(r, a.factor);
@@ -328,11 +347,11 @@ __global__ void __launch_bounds__(512, 2) rows_block_kernel(const T* __restrict_
     if (gz == nullptr) return;
     __syncthreads();
     const RowGrad<float> g = shared;
-    part.grad(out, shift, same, a.v, first, blockDim.x, g, a.factor);
+    part.grad(out, shift, same, v, first, blockDim.x, g, a.factor);
     const int64_t act = a.actions[i];
-    if (act >= 0 && act < a.v) {
-        const int64_t k = (act + shift) / VEC - (int64_t)rank * blockDim.x * NV;
-        if (k >= 0 && k < (int64_t)blockDim.x * NV && k % blockDim.x == threadIdx.x) put_action(out, row, act, g, a.factor);
+    if (act >= 0 && act < v) {
+        const int k = ((int)act + shift) / VEC - rank * (int)blockDim.x * NV;
+        if (k >= 0 && k < (int)blockDim.x * NV && k % blockDim.x == threadIdx.x) put_action(out, row, act, g, a.factor);
     }
 }
 
@@ -541,22 +560,22 @@ __global__ void __launch_bounds__(256) rows_grad_kernel(const T* __restrict__ z,
     T* out = gz + i * a.gn;
     const int shift = shift_of(row);
     const bool same = shift_of(out) == shift;
-    const int64_t first = (int64_t)(blockIdx.x % chunks) * blockDim.x * NV + threadIdx.x;
+    const int first = (int)(blockIdx.x % chunks) * blockDim.x * NV + threadIdx.x, v = (int)a.v;
     if (a.mask != nullptr && !a.mask[i]) {
-        RowPart<T, NV>::zero(out, shift, same, a.v, first, blockDim.x);
+        RowPart<T, NV>::zero(out, shift, same, v, first, blockDim.x);
         return;
     }
     RowPart<T, NV> part;
-    part.load(row, shift, a.v, first, blockDim.x);
+    part.load(row, shift, v, first, blockDim.x);
     const int64_t act = a.actions[i];
     float c = (a.slope != nullptr ? a.slope[i] : 1.f) * (a.scale != nullptr ? a.scale[0] : 1.f) *
               (a.upstream != nullptr ? a.upstream[i * a.up_stride] : 1.f) * a.inv_t;
     if (act < 0 || act >= a.v) c = NAN;
     const RowGrad<float> g = {a.stats[i], c, -c / a.stats[a.n + i]};
-    part.grad(out, shift, same, a.v, first, blockDim.x, g, a.factor);
-    if (act >= 0 && act < a.v) {
-        const int64_t k = (act + shift) / RowPart<T, NV>::VEC - (int64_t)(blockIdx.x % chunks) * blockDim.x * NV;
-        if (k >= 0 && k < (int64_t)blockDim.x * NV && k % blockDim.x == threadIdx.x) put_action(out, row, act, g, a.factor);
+    part.grad(out, shift, same, v, first, blockDim.x, g, a.factor);
+    if (act >= 0 && act < v) {
+        const int k = ((int)act + shift) / RowPart<T, NV>::VEC - (int)(blockIdx.x % chunks) * (int)blockDim.x * NV;
+        if (k >= 0 && k < (int)blockDim.x * NV && k % blockDim.x == threadIdx.x) put_action(out, row, act, g, a.factor);
     }
 }
 
@@ -679,6 +698,7 @@ template <typename T> struct Logits {
             return cudaGetLastError();
         }
         if constexpr (sizeof(A) == 4) {
+            if (a.v < (1 << 30)) {
             constexpr int NV = 4;
             const int64_t w = ceil_div64(a.v + 16 / sizeof(T) - 1, 16 / sizeof(T));
             unsigned bx = 4;
@@ -686,10 +706,10 @@ template <typename T> struct Logits {
             const int64_t chunks = ceil_div64(w, bx * NV);
             return launch(rows_grad_kernel<T, NV>, ceil_div64(a.n, 256 / bx) * chunks, dim3(bx, 256 / bx), 1, s, (const T*)z,
                           (T*)gz, a, (unsigned)chunks);
-        } else {
-            logit_grad_kernel<T, false><<<blocks(a.n), 256, 0, s>>>((const T*)z, (T*)gz, a);
-            return cudaGetLastError();
+            }
         }
+        logit_grad_kernel<T, false><<<blocks(a.n), 256, 0, s>>>((const T*)z, (T*)gz, a);
+        return cudaGetLastError();
     }
 
     static int logp(const void* z, int64_t ldz, int64_t n, int64_t v, bool cols, const int64_t* actions,
