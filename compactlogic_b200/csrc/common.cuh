@@ -94,6 +94,18 @@ template <typename A> __device__ __forceinline__ A warp_sum(A v) {
     return v;
 }
 
+// SMs of the current device (148 on a B200), asked once.
+inline int gpu_sms() {
+    static const int n = [] {
+        int dev = 0, k = 0;
+        return cudaGetDevice(&dev) == cudaSuccess &&
+                       cudaDeviceGetAttribute(&k, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess
+                   ? k
+                   : 148;
+    }();
+    return n;
+}
+
 inline int64_t ceil_div64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 }  // namespace clb

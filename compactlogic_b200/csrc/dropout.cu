@@ -275,17 +275,6 @@ __global__ void dropout_advance_kernel(int64_t* state, int64_t* used) {
     state[1] = (int64_t)((uint64_t)state[1] + 1);
 }
 
-int sm_count() {
-    static const int n = [] {
-        int dev = 0, k = 0;
-        return cudaGetDevice(&dev) == cudaSuccess &&
-                       cudaDeviceGetAttribute(&k, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess
-                   ? k
-                   : 148;
-    }();
-    return n;
-}
-
 template <typename T, bool RESCALE>
 cudaError_t launch(const T* x, T* y, const DropArgs& a, bool batch_inner, cudaStream_t s) {
     constexpr int V = 16 / sizeof(T);
@@ -300,7 +289,7 @@ cudaError_t launch(const T* x, T* y, const DropArgs& a, bool batch_inner, cudaSt
     // As many blocks as are resident at once, each walking down the rows; four times that for shifted rows, whose blocks
     // are rounded to whole shifts and would leave SMs idle (fp16 1001 x 16383, both passes: 75 us with one wave, 51 with
     // four, 57 with eight).
-    int64_t most = (int64_t)sm_count() * kBlocks * (wide ? 1 : 4) / gx;
+    int64_t most = (int64_t)gpu_sms() * kBlocks * (wide ? 1 : 4) / gx;
     if (!wide) most -= most % (V / 2);
     if (most < V / 2) most = V / 2;
     const dim3 grid((unsigned)gx, (unsigned)(gy < most ? gy : most));

@@ -47,12 +47,25 @@ template <typename A> struct RowArgs {
     A fixed;
 };
 
-// One row from its maximum and sum; returns d loss_i / d lp_i before the scale.  write: put the results down.
+// The per-row inputs, read before the row's sum is known so that they have arrived by then.
+template <typename A> struct RowIn { A at, adv, old_lp, ref; };
+
 template <typename T, typename A = typename Acc<T>::type>
-__device__ A finish_row(const T* __restrict__ z, const RowArgs<A>& a, int64_t i, A m, A s, bool write = true) {
+__device__ __forceinline__ RowIn<A> row_in(const T* __restrict__ z, const RowArgs<A>& a, int64_t i) {
+    RowIn<A> in{(A)NAN, 0, 0, 0};
     const int64_t act = a.actions[i];
-    A lp = (A)NAN;
-    if (act >= 0 && act < a.v) lp = (to_acc(z[i * a.sn + act * a.sv]) - m) * a.inv_t - log(s);
+    if (a.adv != nullptr) {
+        in.adv = a.adv[i];
+        in.old_lp = a.old_lp[i];
+        if (a.ref != nullptr) in.ref = a.ref[i];
+    }
+    if (act >= 0 && act < a.v) in.at = to_acc(z[i * a.sn + act * a.sv]);
+    return in;
+}
+
+// One row from its maximum and sum; returns d loss_i / d lp_i before the scale.  write: put the results down.
+template <typename A> __device__ A finish_row(const RowArgs<A>& a, const RowIn<A>& in, int64_t i, A m, A s, bool write) {
+    const A lp = (in.at - m) * a.inv_t - log(s);
     if (write) {
         a.logp[i] = lp;
         if (a.stats != nullptr) {
@@ -61,14 +74,14 @@ __device__ A finish_row(const T* __restrict__ z, const RowArgs<A>& a, int64_t i,
         }
     }
     if (a.adv == nullptr) return (A)0;
-    const A adv = a.adv[i], r = exp(lp - a.old_lp[i]);
+    const A r = exp(lp - in.old_lp);
     const A held = r < a.lo ? a.lo : r > a.hi ? a.hi : r;  // NaN stays NaN
-    const A free_ = r * adv, kept = held * adv;
+    const A free_ = r * in.adv, kept = held * in.adv;
     A loss = -(free_ <= kept ? free_ : kept), slope = free_ <= kept ? -free_ : (A)0;
     if (free_ != free_) loss = slope = free_;
     A kl = 0;
     if (a.ref != nullptr) {
-        const A q = a.ref[i] - lp, e = expm1(q);
+        const A q = in.ref - lp, e = expm1(q);
         kl = e - q;
         loss += a.beta * kl;
         slope -= a.beta * e;
@@ -113,12 +126,19 @@ template <typename A> struct Run {
     }
 };
 
-template <typename A> __device__ __forceinline__ void warp_merge(Run<A>& r, A factor) {
+// The runs of a warp's lanes, G at a time, as one: the common maximum first, so that each sum is rescaled once.
+template <int G = 32, typename A> __device__ __forceinline__ void warp_merge(Run<A>& r, A factor) {
+    A top = r.m;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const A m2 = __shfl_xor_sync(0xffffffffu, r.m, o), s2 = __shfl_xor_sync(0xffffffffu, r.s, o);
-        r.merge(m2, s2, factor);
+    for (int o = G / 2; o > 0; o >>= 1) {
+        const A m2 = __shfl_xor_sync(0xffffffffu, top, o);
+        top = top > m2 ? top : m2;
     }
+    const A safe = top == lowest<A>() ? (A)0 : top;
+    r.s *= soft_exp((r.m - safe) * factor);
+    r.m = top;
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1) r.s += __shfl_xor_sync(0xffffffffu, r.s, o);
 }
 
 // What a row's gradient needs beside its logits: gz_j = c [j = act] + w exp((z_j - m) / T) with w = -c / s.
@@ -264,19 +284,17 @@ __global__ void __launch_bounds__(128) rows_group_kernel(const T* __restrict__ z
     const int shift = shift_of(row);
     RowPart<T, NV> part;
     Run<float> r;
+    RowIn<float> given{};
     if (live) {
+        if (lane == 0) given = row_in<T>(z, a, i);
         part.load(row, shift, v, lane, G);
         part.sum(r, a.factor);
     }
-#pragma unroll
-    for (int o = G / 2; o > 0; o >>= 1) {
-        const float m2 = __shfl_xor_sync(0xffffffffu, r.m, o), s2 = __shfl_xor_sync(0xffffffffu, r.s, o);
-        r.merge(m2, s2, a.factor);
-    }
+    warp_merge<G>(r, a.factor);
     float slope = 0.f;
     if (lane == 0 && in) {
         if (live)
-            slope = finish_row<T>(z, a, i, r.m, r.s);
+            slope = finish_row(a, given, i, r.m, r.s, true);
         else
             skip_row(a, i);
     }
@@ -317,6 +335,8 @@ __global__ void __launch_bounds__(512, 2) rows_block_kernel(const T* __restrict_
         return;
     }
     if (parts > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // this block has started
+    RowIn<float> given{};
+    if (threadIdx.x == 0) given = row_in<T>(z, a, i);
     RowPart<T, NV> part;
     part.load(row, shift, v, first, blockDim.x);
     Run<float> r;
@@ -340,7 +360,7 @@ __global__ void __launch_bounds__(512, 2) rows_block_kernel(const T* __restrict_
         for (int k = lane; k < parts * warps; k += 32) t.merge(runs[k].x, runs[k].y, a.factor);
         warp_merge(t, a.factor);
         if (lane == 0) {
-            const float slope = finish_row<T>(z, a, i, t.m, t.s, rank == 0);
+            const float slope = finish_row(a, given, i, t.m, t.s, rank == 0);
             if (gz != nullptr) shared = row_grad(a, slope, t.m, t.s);
         }
     }
@@ -390,7 +410,7 @@ __global__ void __launch_bounds__(512) rows_stream_kernel(const T* __restrict__ 
         __syncthreads();
         if (threadIdx.x == 0) {
             for (int w = 1; w < (int)(blockDim.x >> 5); ++w) r.merge(sm[w], ss[w], a.factor);
-            const A slope = finish_row<T>(z, a, i, r.m, r.s);
+            const A slope = finish_row(a, row_in<T>(z, a, i), i, r.m, r.s, true);
             if (gz != nullptr) shared = row_grad(a, slope, r.m, r.s);
         }
         if (gz == nullptr) continue;
@@ -426,6 +446,8 @@ __global__ void __launch_bounds__(512) cols_kernel(const T* __restrict__ z, T* _
     if (parts > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     Run<A> r;
     A f[R];
+    RowIn<A> given{};
+    if (live && threadIdx.y == 0) given = row_in<T>(z, a, i);
     if (live) {
         for (int64_t j = first; j < a.v; j += (int64_t)R * stride) {
 #pragma unroll
@@ -473,7 +495,7 @@ __global__ void __launch_bounds__(512) cols_kernel(const T* __restrict__ z, T* _
                 r = Run<A>();
                 for (int w = 0; w < stride; ++w) r.merge(sm[w][threadIdx.x], ss[w][threadIdx.x], a.factor);
             }
-            const A slope = finish_row<T>(z, a, i, r.m, r.s, rank == 0);
+            const A slope = finish_row(a, given, i, r.m, r.s, rank == 0);
             if (gz != nullptr) shared[threadIdx.x] = row_grad(a, slope, r.m, r.s);
         } else if (rank == 0) {
             skip_row(a, i);
@@ -633,6 +655,10 @@ unsigned blocks(int64_t n) { return (unsigned)(n < (1 << 30) ? n : (1 << 30)); }
 
 template <typename P> struct Same { using type = P; };  // a parameter that is not deduced
 
+// Threads of a block of rows_block_kernel; twice as many where eight such blocks do not hold a row.  Blocks of 256 threads
+// hold 32 KB of a row and four of them an SM's registers; with 512 (two an SM) bf16 2048 x 131072 takes 267 us, with 256 262.
+constexpr int kBlockMost = 256;
+
 template <typename T> struct Logits {
     using A = typename Acc<T>::type;
 
@@ -682,11 +708,12 @@ template <typename T> struct Logits {
             if (w <= 64) return group(rows_group_kernel<T, 2, 32>, 32);
             if (w <= 128) return group(rows_group_kernel<T, 4, 32>, 32);
             auto threads = [](int64_t k) { return dim3((unsigned)(ceil_div64(k, 32) * 32)); };
-            if (w <= 4 * 512) return launch(rows_block_kernel<T, 4>, a.n, threads(ceil_div64(w, 4)), 1, s, z, gz, a, 1);
-            for (int parts = 1; parts <= 8; parts *= 2)
-                if (w <= (int64_t)parts * 8 * 512)
-                    return launch(rows_block_kernel<T, 8>, a.n * parts, threads(ceil_div64(w, 8 * parts)), parts, s, z, gz, a,
-                                  parts);
+            if (w <= 4 * kBlockMost) return launch(rows_block_kernel<T, 4>, a.n, threads(ceil_div64(w, 4)), 1, s, z, gz, a, 1);
+            for (int most = kBlockMost; most <= 2 * kBlockMost; most *= 2)
+                for (int parts = 1; parts <= 8; parts *= 2)
+                    if (w <= (int64_t)parts * 8 * most)
+                        return launch(rows_block_kernel<T, 8>, a.n * parts, threads(ceil_div64(w, 8 * parts)), parts, s, z, gz,
+                                      a, parts);
         }
         return launch(rows_stream_kernel<T>, a.n, dim3(512), 1, s, z, gz, a);
     }
