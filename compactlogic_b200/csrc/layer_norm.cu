@@ -200,31 +200,36 @@ __global__ void __launch_bounds__(256) norm_weight_cols_kernel(const T* __restri
 // ---- rows held in registers (fp32 / bf16 / fp16) ----
 // G threads own a row (of `parts` blocks of a cluster: a contiguous share of it), E entries each, and walk down the rows
 // with the next row's loads in flight; weight, bias and the weight's gradients of a thread's columns stay in its registers
-// all the way.  ALIGNED: rows start on 16 bytes and hold whole 16-byte packs, thread t owns packs t, t + G, ...; else single
-// elements t, t + G, ..., which stay coalesced whatever the rows' alignment.
+// all the way.  A row is cut into 16-byte windows from the last 16-byte boundary before it, `shift` entries back; thread t of
+// a share owns windows t, t + G, ...  The rows of one thread are a multiple of a whole pack's entries apart, so their shift
+// is the same and a thread's columns do not move.
 
-template <typename T, int E, bool ALIGNED> struct Line {
+template <typename T> __device__ __forceinline__ int shift_of(const T* p) {
+    return (int)((reinterpret_cast<uintptr_t>(p) / sizeof(T)) % (16 / sizeof(T)));
+}
+
+template <typename T, int E> struct Line {
     static constexpr int VEC = 16 / sizeof(T);
     Pack<T, VEC> p[E / VEC];
 
-    static __device__ __forceinline__ int column(int e, int t, int g) {
-        return ALIGNED ? (e / VEC * g + t) * VEC + e % VEC : e * g + t;
-    }
-    __device__ __forceinline__ void load(const T* __restrict__ row, int t, int g, int d) {
-        if constexpr (ALIGNED) {
+    // column of entry e, with c0 = column of the thread's first window (negative before the row)
+    static __device__ __forceinline__ int column(int e, int c0, int g) { return c0 + e / VEC * g * VEC + e % VEC; }
+
+    // d = 0: nothing, all zeros.  wide: the row's windows are whole 16-byte words of memory
+    __device__ __forceinline__ void load(const T* __restrict__ row, int c0, int g, int d, bool wide) {
+        const unsigned whole = wide && d >= VEC ? d - VEC + 1 : 0;
 #pragma unroll
-            for (int u = 0; u < E / VEC; ++u) {
-                const int c = (u * g + t) * VEC;
-                if (c < d)
-                    p[u].load(row + c);
-                else
-                    p[u] = {};
-            }
-        } else {
+        for (int u = 0; u < E / VEC; ++u) {
+            const int c = c0 + u * g * VEC;
+            if ((unsigned)c < whole) {
+                p[u].load(row + c);
+            } else {
+                p[u] = {};
+                if (c < d && c + VEC > 0) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const int c = e * g + t;
-                p[e / VEC].raw(e % VEC, c < d ? row[c] : T(0.f));
+                    for (int j = 0; j < VEC; ++j)
+                        if ((unsigned)(c + j) < (unsigned)d) p[u].raw(j, row[c + j]);
+                }
             }
         }
     }
@@ -237,25 +242,23 @@ template <typename T, int E, bool ALIGNED> struct Line {
             for (int j = 0; j < VEC; ++j) f[u * VEC + j] = v[j];
         }
     }
-    static __device__ __forceinline__ void store(T* __restrict__ row, int t, int g, int d, const float (&f)[E]) {
+    static __device__ __forceinline__ void store(T* __restrict__ row, int c0, int g, int d, bool wide, const float (&f)[E]) {
+        const unsigned whole = wide && d >= VEC ? d - VEC + 1 : 0;
 #pragma unroll
         for (int u = 0; u < E / VEC; ++u) {
-            if constexpr (ALIGNED) {
-                const int c = (u * g + t) * VEC;
-                if (c < d) {
-                    float v[VEC];
+            const int c = c0 + u * g * VEC;
+            if (c >= d) break;
+            float v[VEC];
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) v[j] = f[u * VEC + j];
-                    Pack<T, VEC> q;
-                    q.put(v);
-                    q.store(row + c);
-                }
+            for (int j = 0; j < VEC; ++j) v[j] = f[u * VEC + j];
+            Pack<T, VEC> q;
+            q.put(v);
+            if ((unsigned)c < whole) {
+                q.store(row + c);
             } else {
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    const int c = (u * VEC + j) * g + t;
-                    if (c < d) row[c] = from_acc<T>(f[u * VEC + j]);
-                }
+                for (int j = 0; j < VEC; ++j)
+                    if ((unsigned)(c + j) < (unsigned)d) row[c + j] = q.raw(j);
             }
         }
     }
@@ -290,62 +293,71 @@ __device__ __forceinline__ void cluster_share(float2* slots, float2 v, int rank,
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-template <typename T, int E, bool ALIGNED>
+template <typename T, int E>
 __global__ void __launch_bounds__(kMostThreads) norm_line_kernel(const T* __restrict__ x, T* __restrict__ y, NormArgs<float> a,
                                                                  RowPlan plan) {
-    using L = Line<T, E, ALIGNED>;
+    using L = Line<T, E>;
     __shared__ float sums[kMostThreads / 32], squares[kMostThreads / 32];
     __shared__ float2 shares[2][kMostParts];
     const int g = plan.g, t = threadIdx.x % g, rank = (int)(blockIdx.x % (unsigned)plan.parts);
-    const int share = g * E, all = (int)a.d;
-    const int off = rank * share, d = min(max(all - off, 0), share);  // this block's columns of a row
+    const int share = g * E, d = (int)a.d;
     if (plan.parts > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    const int64_t step = (int64_t)(gridDim.x / (unsigned)plan.parts) * plan.rows;
+    int64_t i = (int64_t)(blockIdx.x / (unsigned)plan.parts) * plan.rows + threadIdx.x / g;
+    const int shift = shift_of(x + i * a.sn), c0 = rank * share + t * L::VEC - shift;
+    const bool same = shift_of(y + i * a.gn) == shift;
+    // entries of the row in block k's share
+    auto count = [&](int k) { return min(max(d + shift - k * share, 0), share) - (k == 0 ? shift : 0); };
     float w[E], b[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-        const int c = L::column(e, t, g);
-        w[e] = c < d && a.weight != nullptr ? a.weight[off + c] : 1.f;
-        b[e] = c < d && a.bias != nullptr ? a.bias[off + c] : 0.f;
+        const int c = L::column(e, c0, g);
+        const bool in = (unsigned)c < (unsigned)d;
+        w[e] = in && a.weight != nullptr ? a.weight[c] : 1.f;
+        b[e] = in && a.bias != nullptr ? a.bias[c] : 0.f;
     }
-    const int64_t step = (int64_t)(gridDim.x / (unsigned)plan.parts) * plan.rows;
-    int64_t i = (int64_t)(blockIdx.x / (unsigned)plan.parts) * plan.rows + threadIdx.x / g;
     L next;
-    next.load(x + (i < a.n ? i : 0) * a.sn + off, t, g, i < a.n ? d : 0);
+    next.load(x + (i < a.n ? i : 0) * a.sn, c0, g, i < a.n ? d : 0, true);
     if (plan.parts > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     // every thread of a block takes the same turns, also where its row lies past the end
     for (int64_t top = i - threadIdx.x / g, turn = 0; top < a.n; top += step, i += step, ++turn) {
         float f[E];
         next.get(f);
         const int64_t below = i + step;
-        next.load(x + (below < a.n ? below : 0) * a.sn + off, t, g, below < a.n ? d : 0);
+        next.load(x + (below < a.n ? below : 0) * a.sn, c0, g, below < a.n ? d : 0, true);
         float s = 0;
 #pragma unroll
         for (int e = 0; e < E; ++e) s += f[e];
-        float mu = group_sum(s, sums, g) / (float)max(d, 1);
+        float mu = group_sum(s, sums, g) / (float)max(count(rank), 1);
         float q = 0;
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const float c = L::column(e, t, g) < d ? f[e] - mu : 0.f;
-            q += c * c;
+        for (int u = 0; u < E / L::VEC; ++u) {
+            const int c = c0 + u * g * L::VEC;
+            const bool whole = c >= 0 && c + L::VEC <= d;
+#pragma unroll
+            for (int j = 0; j < L::VEC; ++j) {
+                const float v = f[u * L::VEC + j] - mu;
+                if (whole || (unsigned)(c + j) < (unsigned)d) q = fmaf(v, v, q);
+            }
         }
         q = group_sum(q, squares, g);
         if (plan.parts > 1) {
             float2* slots = shares[turn & 1];
             cluster_share(slots, make_float2(mu, q), rank, plan.parts);
             float m = 0;
-            for (int k = 0; k < plan.parts; ++k) m += slots[k].x * ((float)min(max(all - k * share, 0), share) / (float)all);
+            for (int k = 0; k < plan.parts; ++k) m += slots[k].x * ((float)count(k) / (float)d);
             q = 0;
             for (int k = 0; k < plan.parts; ++k) {
                 const float c = slots[k].x - m;
-                q += slots[k].y + c * c * (float)min(max(all - k * share, 0), share);
+                q += slots[k].y + c * c * (float)count(k);
             }
             mu = m;
         }
-        const float r = 1.f / sqrtf(q / (float)all + a.eps);
+        const float r = 1.f / sqrtf(q / (float)d + a.eps);
         if (i < a.n) {
 #pragma unroll
             for (int e = 0; e < E; ++e) f[e] = fmaf((f[e] - mu) * r, w[e], b[e]);
-            L::store(y + i * a.gn + off, t, g, d, f);
+            L::store(y + i * a.gn, c0, g, d, same, f);
             if (t == 0 && rank == 0) {
                 if (a.mean != nullptr) a.mean[i] = mu;
                 if (a.rstd != nullptr) a.rstd[i] = r;
@@ -355,45 +367,44 @@ __global__ void __launch_bounds__(kMostThreads) norm_line_kernel(const T* __rest
 }
 
 // part: [2, gridDim.x / parts * rows, d] sums of gy h and gy over a group's rows (null: not wanted).  gx null: not wanted.
-template <typename T, int E, bool ALIGNED>
+template <typename T, int E>
 __global__ void __launch_bounds__(kMostThreads) norm_line_grad_kernel(const T* __restrict__ x, const T* __restrict__ gy,
                                                                       T* __restrict__ gx, NormArgs<float> a, RowPlan plan,
                                                                       float* __restrict__ part) {
-    using L = Line<T, E, ALIGNED>;
-    __shared__ float first[2][kMostThreads / 32], second[2][kMostThreads / 32];
+    using L = Line<T, E>;
+    __shared__ float2 sums[2][kMostThreads / 32];
     __shared__ float2 shares[2][kMostParts];
-    const int g = plan.g, t = threadIdx.x % g, rank = (int)(blockIdx.x % (unsigned)plan.parts);
-    const int share = g * E, all = (int)a.d;
-    const int off = rank * share, d = min(max(all - off, 0), share);
+    const int g = plan.g, t = threadIdx.x % g, rank = (int)(blockIdx.x % (unsigned)plan.parts), d = (int)a.d;
     if (plan.parts > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-    float w[E], gw[E] = {}, gb[E] = {};
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const int c = L::column(e, t, g);
-        w[e] = c < d && a.weight != nullptr ? a.weight[off + c] : 1.f;
-    }
-    const float per = 1.f / (float)all;
     const int64_t step = (int64_t)(gridDim.x / (unsigned)plan.parts) * plan.rows;
     const int64_t group = (int64_t)(blockIdx.x / (unsigned)plan.parts) * plan.rows + threadIdx.x / g;
     int64_t i = group;
+    const int shift = shift_of(x + i * a.sn), c0 = (rank * g * (E / L::VEC) + t) * L::VEC - shift;
+    const bool wide = shift_of(gy + i * a.gn) == shift, same = gx != nullptr && shift_of(gx + i * a.on) == shift;
+    float w[E], gw[E] = {}, gb[E] = {};
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const int c = L::column(e, c0, g);
+        w[e] = (unsigned)c < (unsigned)d && a.weight != nullptr ? a.weight[c] : 1.f;
+    }
+    const float per = 1.f / (float)d;
     L xn, gn;
     float mun = 0, rn = 0;
     auto fetch = [&](int64_t k) {
         const bool in = k < a.n;
-        xn.load(x + (in ? k : 0) * a.sn + off, t, g, in ? d : 0);
-        gn.load(gy + (in ? k : 0) * a.gn + off, t, g, in ? d : 0);
+        xn.load(x + (in ? k : 0) * a.sn, c0, g, in ? d : 0, true);
+        gn.load(gy + (in ? k : 0) * a.gn, c0, g, in ? d : 0, wide);
         mun = in ? a.mean[k] : 0.f;
         rn = in ? a.rstd[k] : 0.f;
     };
     fetch(i);
     if (plan.parts > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     for (int64_t top = i - threadIdx.x / g, turn = 0; top < a.n; top += step, i += step, ++turn) {
-        const L xi = xn, gi = gn;
+        float h[E], f[E];
+        xn.get(h);
+        gn.get(f);
         const float mu = mun, r = rn;
         fetch(i + step);
-        float h[E], f[E];
-        xi.get(h);
-        gi.get(f);
         float s1 = 0, s2 = 0;
 #pragma unroll
         for (int e = 0; e < E; ++e) {  // entries past the row have f = 0
@@ -408,16 +419,14 @@ __global__ void __launch_bounds__(kMostThreads) norm_line_grad_kernel(const T* _
         s1 = warp_sum(s1);
         s2 = warp_sum(s2);
         if (g > 32) {
-            const int nw = g >> 5, warp = threadIdx.x >> 5, b = (int)(turn & 1);
-            if ((threadIdx.x & 31) == 0) {
-                first[b][warp] = s1;
-                second[b][warp] = s2;
-            }
+            const int nw = g >> 5, warp = threadIdx.x >> 5;
+            float2* at = sums[turn & 1];
+            if ((threadIdx.x & 31) == 0) at[warp] = make_float2(s1, s2);
             __syncthreads();
             s1 = s2 = 0;
             for (int k = warp / nw * nw, end = k + nw; k < end; ++k) {
-                s1 += first[b][k];
-                s2 += second[b][k];
+                s1 += at[k].x;
+                s2 += at[k].y;
             }
         }
         if (plan.parts > 1) {
@@ -434,38 +443,38 @@ __global__ void __launch_bounds__(kMostThreads) norm_line_grad_kernel(const T* _
         if (i < a.n) {
 #pragma unroll
             for (int e = 0; e < E; ++e) f[e] = r * (f[e] - fmaf(h[e], s2, s1));
-            L::store(gx + i * a.on + off, t, g, d, f);
+            L::store(gx + i * a.on, c0, g, d, same, f);
         }
     }
     if (part == nullptr) return;
-    const int64_t groups = step;
-    float* at = part + group * a.d + off;
+    float* at = part + group * d;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-        const int c = L::column(e, t, g);
-        if (c < d) {
+        const int c = L::column(e, c0, g);
+        if ((unsigned)c < (unsigned)d) {
             at[c] = gw[e];
-            at[groups * a.d + c] = gb[e];
+            at[step * d + c] = gb[e];
         }
     }
 }
 
-// out[j] = sum over p of part[p, j], in a fixed order: 32 columns x 32 shares of the rows a block; blockIdx.y picks gw or gb.
-__global__ void __launch_bounds__(1024) norm_fold_kernel(const float* __restrict__ part, int64_t groups, int64_t d, float* gw,
-                                                         float* gb) {
+// out[j] = sum over p of part[p * ld + j] for j < d, in a fixed order: 32 columns x 32 shares of the rows a block;
+// blockIdx.y picks the first or the second `groups` rows, and gw or gb.
+__global__ void __launch_bounds__(1024) norm_fold_kernel(const float* __restrict__ part, int64_t groups, int64_t ld, int64_t d,
+                                                         float* gw, float* gb) {
     __shared__ float sh[32][33];
     float* out = blockIdx.y == 0 ? gw : gb;
     if (out == nullptr) return;
-    part += blockIdx.y * groups * d;
+    part += blockIdx.y * groups * ld;
     const int64_t j = (int64_t)blockIdx.x * 32 + threadIdx.x;
     float s[4] = {};
     if (j < d) {
         int64_t p = threadIdx.y;
         for (; p + 96 < groups; p += 128) {
 #pragma unroll
-            for (int u = 0; u < 4; ++u) s[u] += part[(p + 32 * u) * d + j];
+            for (int u = 0; u < 4; ++u) s[u] += part[(p + 32 * u) * ld + j];
         }
-        for (; p < groups; p += 32) s[0] += part[p * d + j];
+        for (; p < groups; p += 32) s[0] += part[p * ld + j];
     }
     sh[threadIdx.y][threadIdx.x] = (s[0] + s[1]) + (s[2] + s[3]);
     __syncthreads();
@@ -481,8 +490,9 @@ struct LinePlan {
     int64_t groups;
 };
 
-LinePlan line_plan(int64_t n, int64_t d, int vec, bool backward) {
+LinePlan line_plan(int64_t n, int64_t d, int vec, bool shifted, bool backward) {
     LinePlan p{};
+    if (shifted) d += vec - 1;  // room for the furthest shift
     for (int e = vec; e <= 16; e *= 2)
         if (d <= 32 * e || e == 16) {
             p.e = e;
@@ -502,6 +512,8 @@ LinePlan line_plan(int64_t n, int64_t d, int vec, bool backward) {
     int64_t blocks = (int64_t)gpu_sms() * (threads / (p.plan.g * p.plan.rows)) / p.plan.parts;
     const int64_t most = ceil_div64(n, p.plan.rows);
     blocks = blocks < 1 ? 1 : blocks;
+    // rows of one thread a multiple of a pack's entries apart (see above), where it has more than one
+    if (shifted && blocks < most && blocks % vec != 0) blocks = blocks > vec ? blocks - blocks % vec : vec;
     p.groups = (blocks < most ? blocks : most) * p.plan.rows;
     return p;
 }
@@ -526,25 +538,420 @@ template <typename... P> cudaError_t launch_lines(void (*kernel)(P...), const Li
 
 unsigned blocks(int64_t n) { return (unsigned)(n < (1 << 30) ? n : (1 << 30)); }
 
+// ---- samples contiguous (fp32 / bf16 / fp16) ----
+// The statistics run down the strided axis, the weight's gradients along the contiguous one.  First pass: a warp owns a
+// strip of 32 V samples (V a 16-byte pack, or 1 where rows do not start on 16 bytes) and walks down features 8 at a time,
+// all 8 loads in flight; the blocks of `chunk` features leave partial results, which a small kernel folds.  Second pass:
+// elementwise, reading the operands again.  A call runs both passes over one slab of samples after the other, as many as
+// leave a slab's operands in the L2 cache, so that the second pass does not read memory again.
+
+constexpr int kColThreads = 256, kBatch = 8;
+
+// V consecutive samples of one feature as floats; `left` of them exist.
+template <typename T, int V> struct Strip {
+    uint32_t w[V * sizeof(T) >= 4 ? V * sizeof(T) / 4 : 1];
+    __device__ __forceinline__ void load(const T* __restrict__ p, int left) {
+        if constexpr (V == 1) {
+            T v = left > 0 ? *p : T(0.f);
+            if constexpr (sizeof(T) == 2)
+                w[0] = *reinterpret_cast<const unsigned short*>(&v);
+            else
+                w[0] = *reinterpret_cast<const uint32_t*>(&v);
+        } else {
+            Pack<T, V> q = {};
+            if (left >= V) {
+                q.load(p);
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                    if (j < left) q.raw(j, p[j]);
+            }
+#pragma unroll
+            for (int k = 0; k < Pack<T, V>::kWords; ++k) w[k] = q.w[k];
+        }
+    }
+    __device__ __forceinline__ void get(float (&f)[V]) const {
+        if constexpr (V == 1) {
+            if constexpr (sizeof(T) == 2) {
+                const unsigned short h = (unsigned short)w[0];
+                f[0] = to_acc(*reinterpret_cast<const T*>(&h));
+            } else {
+                f[0] = *reinterpret_cast<const float*>(&w[0]);
+            }
+        } else {
+            Pack<T, V> q;
+#pragma unroll
+            for (int k = 0; k < Pack<T, V>::kWords; ++k) q.w[k] = w[k];
+            q.get(f);
+        }
+    }
+    static __device__ __forceinline__ void store(T* __restrict__ p, int left, const float (&f)[V]) {
+        if constexpr (V == 1) {
+            if (left > 0) *p = from_acc<T>(f[0]);
+        } else {
+            Pack<T, V> q;
+            q.put(f);
+            if (left >= V) {
+                q.store(p);
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                    if (j < left) p[j] = q.raw(j);
+            }
+        }
+    }
+};
+
+// mean and sum of squared differences of n more values (m, q) joined to those of n0
+__device__ __forceinline__ void join(float& mean, float& m2, float m, float q, float part, float both) {
+    const float c = m - mean;            // part = n / (n0 + n), both = n0 n / (n0 + n)
+    mean = fmaf(c, part, mean);
+    m2 = fmaf(c * c, both, m2 + q);
+}
+
+// stats [2, chunks, n]: mean and sum of squared differences of each chunk's features, for the samples from `from` on.
+template <typename T, int V>
+__global__ void __launch_bounds__(kColThreads) norm_strip_stats_kernel(const T* __restrict__ x, NormArgs<float> a,
+                                                                       int64_t from, int64_t to, int64_t chunk,
+                                                                       float* __restrict__ stats) {
+    constexpr int W = kColThreads / 32;
+    __shared__ float sh[W][2][32 * V];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t i = from + ((int64_t)blockIdx.x * 32 + lane) * V, j0 = blockIdx.y * chunk;
+    const int left = (int)(to - i < V ? (to > i ? to - i : 0) : V);
+    const int64_t end = j0 + chunk < a.d ? j0 + chunk : a.d;
+    float mean[V] = {}, m2[V] = {};
+    int64_t n = 0;
+    for (int64_t j = j0 + warp * kBatch; j < end; j += W * kBatch) {
+        const int k = (int)(end - j < kBatch ? end - j : kBatch);
+        Strip<T, V> v[kBatch];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u)
+            if (u < k) v[u].load(x + (j + u) * a.sd + i, left);
+        const float per = 1.f / (float)k, part = (float)k / (float)(n + k), both = (float)n * part;
+        float m[V] = {}, q[V] = {};
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u)
+            if (u < k) {
+                float f[V];
+                v[u].get(f);
+#pragma unroll
+                for (int c = 0; c < V; ++c) m[c] += f[c];
+            }
+#pragma unroll
+        for (int c = 0; c < V; ++c) m[c] *= per;
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u)
+            if (u < k) {
+                float f[V];
+                v[u].get(f);
+#pragma unroll
+                for (int c = 0; c < V; ++c) q[c] = fmaf(f[c] - m[c], f[c] - m[c], q[c]);
+            }
+#pragma unroll
+        for (int c = 0; c < V; ++c) join(mean[c], m2[c], m[c], q[c], part, both);
+        n += k;
+    }
+#pragma unroll
+    for (int c = 0; c < V; ++c) {
+        sh[warp][0][c * 32 + lane] = mean[c];
+        sh[warp][1][c * 32 + lane] = m2[c];
+    }
+    __syncthreads();
+    // features warp k has walked over: whole batches from its first on, W batches apart
+    for (int c = threadIdx.x; c < 32 * V; c += kColThreads) {
+        const int64_t at = from + (int64_t)blockIdx.x * 32 * V + (c % 32) * V + c / 32;
+        float m = 0, q = 0;
+        int64_t n0 = 0;
+        for (int k = 0; k < W; ++k) {
+            int64_t nk = 0;
+            for (int64_t j = j0 + k * kBatch; j < end; j += W * kBatch) nk += end - j < kBatch ? end - j : kBatch;
+            if (nk == 0) break;
+            const float part = (float)nk / (float)(n0 + nk);
+            join(m, q, sh[k][0][c], sh[k][1][c], part, (float)n0 * part);
+            n0 += nk;
+        }
+        if (at < to) {
+            stats[blockIdx.y * a.n + at] = m;
+            stats[(gridDim.y + blockIdx.y) * a.n + at] = q;
+        }
+    }
+}
+
+// mean and rstd from the chunks: 32 samples x 8 shares of the chunks a block
+__global__ void __launch_bounds__(256) norm_strip_fold_kernel(const float* __restrict__ stats, int64_t n, int64_t d,
+                                                              int64_t from, int64_t to, int64_t chunk, int chunks, float eps,
+                                                              float* mean, float* rstd) {
+    __shared__ float sh[8][3][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t i = from + (int64_t)blockIdx.x * 32 + lane;
+    float m = 0, q = 0, n0 = 0;
+    if (i < to)
+        for (int k = warp; k < chunks; k += 8) {
+            const float nk = (float)(d - k * chunk < chunk ? d - k * chunk : chunk), part = nk / (n0 + nk);
+            join(m, q, stats[k * n + i], stats[(chunks + k) * n + i], part, n0 * part);
+            n0 += nk;
+        }
+    sh[warp][0][lane] = m;
+    sh[warp][1][lane] = q;
+    sh[warp][2][lane] = n0;
+    __syncthreads();
+    if (warp != 0 || i >= to) return;
+    for (int k = 1; k < 8; ++k) {
+        const float nk = sh[k][2][lane];
+        if (nk == 0) break;
+        const float part = nk / (n0 + nk);
+        join(m, q, sh[k][0][lane], sh[k][1][lane], part, n0 * part);
+        n0 += nk;
+    }
+    mean[i] = m;
+    rstd[i] = 1.f / sqrtf(q / (float)d + eps);
+}
+
+// y from x, mean and rstd; or gx from x, gy, and the folded sums c1, c2 (GRAD)
+template <typename T, int V, bool GRAD>
+__global__ void __launch_bounds__(kColThreads) norm_strip_apply_kernel(const T* __restrict__ x, const T* __restrict__ gy,
+                                                                       T* __restrict__ y, NormArgs<float> a, int64_t from,
+                                                                       int64_t to, int64_t chunk, const float* mean,
+                                                                       const float* rstd, const float* c1, const float* c2) {
+    constexpr int W = kColThreads / 32, B = GRAD ? 4 : 8;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t i = from + ((int64_t)blockIdx.x * 32 + lane) * V, j0 = blockIdx.y * chunk;
+    const int left = (int)(to - i < V ? (to > i ? to - i : 0) : V);
+    const int64_t end = j0 + chunk < a.d ? j0 + chunk : a.d, ld = GRAD ? a.od : a.gd;
+    if (left == 0) return;
+    float mu[V], r[V], k1[V], k2[V];
+    const float per = 1.f / (float)a.d;
+#pragma unroll
+    for (int c = 0; c < V; ++c) {
+        const int64_t at = c < left ? i + c : i;
+        mu[c] = mean[at];
+        r[c] = rstd[at];
+        if (GRAD) {
+            k1[c] = c1[at] * per;
+            k2[c] = c2[at] * per;
+        }
+    }
+    for (int64_t j = j0 + warp * B; j < end; j += W * B) {
+        Strip<T, V> v[B], g[GRAD ? B : 1];
+#pragma unroll
+        for (int u = 0; u < B; ++u)
+            if (j + u < end) {
+                v[u].load(x + (j + u) * a.sd + i, left);
+                if (GRAD) g[u].load(gy + (j + u) * a.gd + i, left);
+            }
+#pragma unroll
+        for (int u = 0; u < B; ++u)
+            if (j + u < end) {
+                float f[V], t[V];
+                v[u].get(f);
+                const float w = a.weight != nullptr ? a.weight[j + u] : 1.f;
+                if constexpr (GRAD) {
+                    g[u].get(t);
+#pragma unroll
+                    for (int c = 0; c < V; ++c)
+                        t[c] = r[c] * (fmaf(t[c], w, -k1[c]) - (f[c] - mu[c]) * r[c] * k2[c]);
+                } else {
+                    const float b = a.bias != nullptr ? a.bias[j + u] : 0.f;
+#pragma unroll
+                    for (int c = 0; c < V; ++c) t[c] = fmaf((f[c] - mu[c]) * r[c], w, b);
+                }
+                Strip<T, V>::store(y + (j + u) * ld + i, left, t);
+            }
+    }
+}
+
+// sums [2, chunks, n]: sum of t and of t h over each chunk's features (t = gy w), by sample; and part [2, strips, d]: sums
+// of gy h and of gy over each strip's samples, by feature (null: not wanted).
+template <typename T, int V>
+__global__ void __launch_bounds__(kColThreads) norm_strip_sums_kernel(const T* __restrict__ x, const T* __restrict__ gy,
+                                                                      NormArgs<float> a, int64_t from, int64_t to,
+                                                                      int64_t chunk, float* __restrict__ sums,
+                                                                      float* __restrict__ part, int64_t strip0,
+                                                                      int64_t strips) {
+    constexpr int W = kColThreads / 32, B = kBatch;
+    __shared__ float sh[W][2][32 * V];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t i = from + ((int64_t)blockIdx.x * 32 + lane) * V, j0 = blockIdx.y * chunk;
+    const int left = (int)(to - i < V ? (to > i ? to - i : 0) : V);
+    const int64_t end = j0 + chunk < a.d ? j0 + chunk : a.d;
+    float mu[V], r[V], s1[V] = {}, s2[V] = {};
+#pragma unroll
+    for (int c = 0; c < V; ++c) {
+        mu[c] = c < left ? a.mean[i + c] : 0.f;
+        r[c] = c < left ? a.rstd[i + c] : 0.f;
+    }
+    for (int64_t j = j0 + warp * B; j < end; j += W * B) {
+        Strip<T, V> v[B], g[B];
+#pragma unroll
+        for (int u = 0; u < B; ++u) {
+            const int have = j + u < end ? left : 0;
+            v[u].load(x + (j + u) * a.sd + i, have);
+            g[u].load(gy + (j + u) * a.gd + i, have);
+        }
+        float both[2 * B];
+#pragma unroll
+        for (int u = 0; u < B; ++u) {
+            float f[V], t[V], p = 0, q = 0;
+            v[u].get(f);
+            g[u].get(t);
+            const float w = a.weight != nullptr && j + u < end ? a.weight[j + u] : 1.f;
+#pragma unroll
+            for (int c = 0; c < V; ++c) {  // samples and features past the end have gy = h = 0
+                const float h = (f[c] - mu[c]) * r[c], th = t[c] * h;
+                p += th;
+                q += t[c];
+                s1[c] = fmaf(t[c], w, s1[c]);
+                s2[c] = fmaf(th, w, s2[c]);
+            }
+            both[u] = p;
+            both[B + u] = q;
+        }
+        if (part != nullptr) {
+            // 2 B sums over the lanes at once: at each step a lane keeps half of them and hands over the rest
+#pragma unroll
+            for (int o = 16, k = B; k >= 1; o >>= 1, k >>= 1) {
+                const bool up = lane & o;
+#pragma unroll
+                for (int u = 0; u < k; ++u) {
+                    const float keep = up ? both[u + k] : both[u], give = up ? both[u] : both[u + k];
+                    both[u] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+                }
+            }
+            const float total = both[0] + __shfl_xor_sync(0xffffffffu, both[0], 1);
+            const int u = lane >> 1;  // which of the 2 B sums this lane holds
+            const int64_t f = j + (u & (B - 1));
+            if ((lane & 1) == 0 && f < end) part[((u >= B ? strips : 0) + strip0 + blockIdx.x) * a.d + f] = total;
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < V; ++c) {
+        sh[warp][0][c * 32 + lane] = s1[c];
+        sh[warp][1][c * 32 + lane] = s2[c];
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < 32 * V; c += kColThreads) {
+        const int64_t at = from + (int64_t)blockIdx.x * 32 * V + (c % 32) * V + c / 32;
+        float p = 0, q = 0;
+        for (int k = 0; k < W; ++k) {
+            p += sh[k][0][c];
+            q += sh[k][1][c];
+        }
+        if (at < to) {
+            sums[blockIdx.y * a.n + at] = p;
+            sums[(gridDim.y + blockIdx.y) * a.n + at] = q;
+        }
+    }
+}
+
+struct ColPlan {
+    int v;                 // samples a thread owns
+    int64_t slab, strips;  // samples of a slab (whole strips), strips of the call
+    int64_t chunk;         // features of a block
+    int chunks;
+};
+
+ColPlan col_plan(int64_t n, int64_t d, int elem, bool wide, bool backward) {
+    ColPlan p{};
+    p.v = wide ? 16 / elem : 1;
+    const int64_t strip = 32 * p.v, all = ceil_div64(n, strip);
+    // Half of the L2 cache for a slab's operands; the whole call where it fits
+    const int64_t room = (int64_t)48 << 20, bytes = d * strip * elem * (backward ? 2 : 1);
+    int64_t per = room / bytes < 1 ? 1 : room / bytes;
+    if (all * bytes <= (int64_t)80 << 20 || bytes > room) per = all;
+    p.slab = per * strip;
+    p.strips = all;
+    const int64_t wanted = ceil_div64((int64_t)gpu_sms() * 3, per < all ? per : all), unit = kColThreads / 32 * kBatch;
+    p.chunk = ceil_div64(ceil_div64(d, wanted), unit) * unit;
+    p.chunks = (int)ceil_div64(d, p.chunk);
+    return p;
+}
+
 template <typename T> struct Norm {
     using A = typename Acc<T>::type;
     static constexpr int VEC = 16 / sizeof(T);
 
-    static bool aligned(const void* p, int64_t ld, const NormArgs<A>& a) {
-        return reinterpret_cast<uintptr_t>(p) % 16 == 0 && a.d % VEC == 0 && (a.n == 1 || ld % VEC == 0);
+    // rows (of the strided axis) that all start on 16 bytes
+    static bool wide(const void* p, int64_t ld, int64_t rows) {
+        return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (rows <= 1 || ld % VEC == 0);
     }
 
-    static cudaError_t forward(const void* x, void* y, const NormArgs<A>& a, bool cols, cudaStream_t s) {
+    static size_t workspace(int64_t n, int64_t d, bool cols, bool backward) {
+        if (sizeof(A) != 4 || n == 0) return 0;
+        int64_t most = 0;
+        for (int k = 0; k < 2; ++k) {  // whichever way the pointers turn out to be aligned
+            if (cols) {
+                const ColPlan p = col_plan(n, d, (int)sizeof(T), k == 0, backward);
+                const int64_t need = 2 * p.chunks * n + 2 * n + (backward ? 2 * p.strips * d : 0);
+                most = need > most ? need : most;
+            } else if (backward) {
+                const LinePlan p = line_plan(n, d, VEC, k == 0, true);
+                const int64_t need = p.e != 0 ? 2 * p.groups * d : 0;
+                most = need > most ? need : most;
+            }
+        }
+        return (size_t)most * sizeof(A);
+    }
+
+    template <int V> static cudaError_t forward_strips(const T* x, T* y, NormArgs<float> a, const ColPlan& p, float* ws,
+                                                       cudaStream_t s) {
+        float* stats = ws + 2 * a.n;
+        if (a.mean == nullptr) a.mean = ws;
+        if (a.rstd == nullptr) a.rstd = ws + a.n;
+        for (int64_t from = 0; from < a.n; from += p.slab) {
+            const int64_t to = from + p.slab < a.n ? from + p.slab : a.n;
+            const dim3 grid((unsigned)ceil_div64(to - from, 32 * V), (unsigned)p.chunks);
+            norm_strip_stats_kernel<T, V><<<grid, kColThreads, 0, s>>>(x, a, from, to, p.chunk, stats);
+            norm_strip_fold_kernel<<<(unsigned)ceil_div64(to - from, 32), 256, 0, s>>>(stats, a.n, a.d, from, to, p.chunk,
+                                                                                     p.chunks, a.eps, a.mean, a.rstd);
+            norm_strip_apply_kernel<T, V, false><<<grid, kColThreads, 0, s>>>(x, nullptr, y, a, from, to, p.chunk, a.mean,
+                                                                              a.rstd, nullptr, nullptr);
+            count_launches(3);
+            const cudaError_t e = cudaGetLastError();
+            if (e != cudaSuccess) return e;
+        }
+        return cudaSuccess;
+    }
+
+    template <int V> static cudaError_t backward_strips(const T* x, const T* gy, T* gx, float* gw, float* gb,
+                                                        const NormArgs<float>& a, const ColPlan& p, float* ws, cudaStream_t s) {
+        float *c1 = ws, *c2 = ws + a.n, *sums = ws + 2 * a.n, *part = sums + 2 * p.chunks * a.n;
+        const bool weights = gw != nullptr || gb != nullptr;
+        for (int64_t from = 0; from < a.n; from += p.slab) {
+            const int64_t to = from + p.slab < a.n ? from + p.slab : a.n;
+            const dim3 grid((unsigned)ceil_div64(to - from, 32 * V), (unsigned)p.chunks);
+            norm_strip_sums_kernel<T, V><<<grid, kColThreads, 0, s>>>(x, gy, a, from, to, p.chunk, sums,
+                                                                      weights ? part : nullptr, from / (32 * V), p.strips);
+            count_launches(1);
+            if (gx != nullptr) {
+                norm_fold_kernel<<<dim3((unsigned)ceil_div64(to - from, 32), 2), dim3(32, 32), 0, s>>>(
+                    sums + from, p.chunks, a.n, to - from, c1 + from, c2 + from);
+                norm_strip_apply_kernel<T, V, true><<<grid, kColThreads, 0, s>>>(x, gy, gx, a, from, to, p.chunk, a.mean,
+                                                                                 a.rstd, c1, c2);
+                count_launches(2);
+            }
+            const cudaError_t e = cudaGetLastError();
+            if (e != cudaSuccess) return e;
+        }
+        if (weights) {
+            norm_fold_kernel<<<dim3((unsigned)ceil_div64(a.d, 32), 2), dim3(32, 32), 0, s>>>(part, p.strips, a.d, a.d, gw, gb);
+            count_launches(1);
+        }
+        return cudaGetLastError();
+    }
+
+    static cudaError_t forward(const void* x, void* y, const NormArgs<A>& a, bool cols, void* ws, cudaStream_t s) {
         if constexpr (sizeof(A) == 4) {
-            const LinePlan p = line_plan(a.n, a.d, VEC, false);
-            if (!cols && p.e != 0) {
-                auto go = [&](auto wide, auto narrow) {
-                    return launch_lines(aligned(x, a.sn, a) && aligned(y, a.gn, a) ? wide : narrow, p, s, (const T*)x, (T*)y, a,
-                                        p.plan);
-                };
-                if (p.e == 16) return go(norm_line_kernel<T, 16, true>, norm_line_kernel<T, 16, false>);
-                if (p.e == 8) return go(norm_line_kernel<T, 8, true>, norm_line_kernel<T, 8, false>);
-                return go(norm_line_kernel<T, VEC, true>, norm_line_kernel<T, VEC, false>);
+            if (cols) {
+                const bool w = wide(x, a.sd, a.d) && wide(y, a.gd, a.d);
+                const ColPlan p = col_plan(a.n, a.d, (int)sizeof(T), w, false);
+                return w ? forward_strips<VEC>((const T*)x, (T*)y, a, p, (float*)ws, s)
+                         : forward_strips<1>((const T*)x, (T*)y, a, p, (float*)ws, s);
+            }
+            const LinePlan p = line_plan(a.n, a.d, VEC, !wide(x, a.sn, a.n), false);
+            if (p.e != 0) {
+                auto go = [&](auto kernel) { return launch_lines(kernel, p, s, (const T*)x, (T*)y, a, p.plan); };
+                return p.e == 16 ? go(norm_line_kernel<T, 16>) : p.e == 8 ? go(norm_line_kernel<T, 8>) : go(norm_line_kernel<T, VEC>);
             }
         }
         count_launches(1);
@@ -555,28 +962,26 @@ template <typename T> struct Norm {
         return cudaGetLastError();
     }
 
-    static size_t workspace(int64_t n, int64_t d, bool cols, bool backward) {
-        if (sizeof(A) != 4 || cols || !backward || n == 0) return 0;
-        const LinePlan p = line_plan(n, d, VEC, true);
-        return p.e != 0 ? (size_t)(2 * p.groups * d) * sizeof(A) : 0;
-    }
-
     static cudaError_t backward(const void* x, const void* gy, void* gx, A* gw, A* gb, const NormArgs<A>& a, bool cols,
-                                void* workspace, cudaStream_t s) {
+                                void* ws, cudaStream_t s) {
         if constexpr (sizeof(A) == 4) {
-            const LinePlan p = line_plan(a.n, a.d, VEC, true);
-            if (!cols && a.n > 0 && p.e != 0) {
-                float* part = gw != nullptr || gb != nullptr ? (float*)workspace : nullptr;
-                auto go = [&](auto wide, auto narrow) {
-                    const bool al = aligned(x, a.sn, a) && aligned(gy, a.gn, a) && (gx == nullptr || aligned(gx, a.on, a));
-                    return launch_lines(al ? wide : narrow, p, s, (const T*)x, (const T*)gy, (T*)gx, a, p.plan, part);
+            if (cols && a.n > 0) {
+                const bool w = wide(x, a.sd, a.d) && wide(gy, a.gd, a.d) && (gx == nullptr || wide(gx, a.od, a.d));
+                const ColPlan p = col_plan(a.n, a.d, (int)sizeof(T), w, true);
+                return w ? backward_strips<VEC>((const T*)x, (const T*)gy, (T*)gx, gw, gb, a, p, (float*)ws, s)
+                         : backward_strips<1>((const T*)x, (const T*)gy, (T*)gx, gw, gb, a, p, (float*)ws, s);
+            }
+            const LinePlan p = line_plan(a.n, a.d, VEC, !wide(x, a.sn, a.n), true);
+            if (a.n > 0 && p.e != 0) {
+                float* part = gw != nullptr || gb != nullptr ? (float*)ws : nullptr;
+                auto go = [&](auto kernel) {
+                    return launch_lines(kernel, p, s, (const T*)x, (const T*)gy, (T*)gx, a, p.plan, part);
                 };
-                const cudaError_t e =
-                    p.e == 16 ? go(norm_line_grad_kernel<T, 16, true>, norm_line_grad_kernel<T, 16, false>)
-                    : p.e == 8 ? go(norm_line_grad_kernel<T, 8, true>, norm_line_grad_kernel<T, 8, false>)
-                               : go(norm_line_grad_kernel<T, VEC, true>, norm_line_grad_kernel<T, VEC, false>);
+                const cudaError_t e = p.e == 16  ? go(norm_line_grad_kernel<T, 16>)
+                                      : p.e == 8 ? go(norm_line_grad_kernel<T, 8>)
+                                                 : go(norm_line_grad_kernel<T, VEC>);
                 if (e != cudaSuccess || part == nullptr) return e;
-                norm_fold_kernel<<<dim3((unsigned)ceil_div64(a.d, 32), 2), dim3(32, 32), 0, s>>>(part, p.groups, a.d, gw, gb);
+                norm_fold_kernel<<<dim3((unsigned)ceil_div64(a.d, 32), 2), dim3(32, 32), 0, s>>>(part, p.groups, a.d, a.d, gw, gb);
                 count_launches(1);
                 return cudaGetLastError();
             }
@@ -665,11 +1070,11 @@ extern "C" int clb_layer_norm_forward(int dtype, const void* x, int64_t ldx, int
     const bool cols = feature_major != 0;
     const auto f = args<float>(n, d, cols, ldx, ldy, 0, weight, bias, eps, mean, rstd);
     switch (dtype) {
-        case CLB_F32: return done(Norm<float>::forward(x, y, f, cols, s));
+        case CLB_F32: return done(Norm<float>::forward(x, y, f, cols, workspace, s));
         case CLB_F64:
-            return done(Norm<double>::forward(x, y, args<double>(n, d, cols, ldx, ldy, 0, weight, bias, eps, mean, rstd), cols, s));
-        case CLB_BF16: return done(Norm<__nv_bfloat16>::forward(x, y, f, cols, s));
-        default: return done(Norm<__half>::forward(x, y, f, cols, s));
+            return done(Norm<double>::forward(x, y, args<double>(n, d, cols, ldx, ldy, 0, weight, bias, eps, mean, rstd), cols, workspace, s));
+        case CLB_BF16: return done(Norm<__nv_bfloat16>::forward(x, y, f, cols, workspace, s));
+        default: return done(Norm<__half>::forward(x, y, f, cols, workspace, s));
     }
 }
 
