@@ -4,6 +4,9 @@
 // Statistics and sums are held in the arithmetic type (fp32; fp64 for fp64 activations).
 #include <cuda_runtime.h>
 
+#include <atomic>
+#include <type_traits>
+
 #include "common.cuh"
 #include "kernels.h"
 #include "vec.cuh"
@@ -197,89 +200,157 @@ __global__ void __launch_bounds__(256) norm_weight_cols_kernel(const T* __restri
     }
 }
 
-// ---- rows held in registers (fp32 / bf16 / fp16) ----
-// G threads own a row (of `parts` blocks of a cluster: a contiguous share of it), E entries each, and walk down the rows
-// with the next row's loads in flight; weight, bias and the weight's gradients of a thread's columns stay in its registers
-// all the way.  A row is cut into 16-byte windows from the last 16-byte boundary before it, `shift` entries back; thread t of
-// a share owns windows t, t + G, ...  The rows of one thread are a multiple of a whole pack's entries apart, so their shift
-// is the same and a thread's columns do not move.
+// ---- rows in 16-byte windows (fp32 / bf16 / fp16) ----
+// G threads own a row (of `parts` blocks of a cluster: a contiguous share of it), NP windows a thread: a warp has 32 NP
+// neighbouring windows, lane l those at l, l + 32, ..., so that a thread's windows are constant distances apart.  A row that
+// does not start on 16 bytes is cut from the last boundary before it, `shift` entries back.  What is known of the windows
+// picks the kernels' form: each is part of the row as a whole (kFull), as a whole or not at all (kWhole: rows start on 16
+// bytes and end with a window), or may be so in part (kShifted).
+//
+// The groups walk down the rows.  The next rows' whole windows travel to shared memory meanwhile (Ring), each thread fetching
+// its own, so that no barrier stands between a copy and its use.  A thread's rows are a multiple of a whole pack's entries
+// apart, so that their shift is the same and its columns do not move.
 
 template <typename T> __device__ __forceinline__ int shift_of(const T* p) {
     return (int)((reinterpret_cast<uintptr_t>(p) / sizeof(T)) % (16 / sizeof(T)));
 }
 
-template <typename T, int E> struct Line {
-    static constexpr int VEC = 16 / sizeof(T);
-    Pack<T, VEC> p[E / VEC];
+enum Windows { kFull, kWhole, kShifted };
+// Rows of a group in shared memory or on their way there: the one at work and the next.  A third would take shared memory
+// from the L1 cache that holds weight and bias (bf16 8192 x 4096, both passes: 101 us with two, 108 with three).
+constexpr int kStages = 2;
 
-    // column of entry e, with c0 = column of the thread's first window (negative before the row)
-    static __device__ __forceinline__ int column(int e, int c0, int g) { return c0 + e / VEC * g * VEC + e % VEC; }
+template <typename T, int NP, Windows M> struct Line {
+    static constexpr int VEC = 16 / sizeof(T), STEP = 32 * VEC;
 
-    // d = 0: nothing, all zeros.  wide: the row's windows are whole 16-byte words of memory
-    __device__ __forceinline__ void load(const T* __restrict__ row, int c0, int g, int d, bool wide) {
-        const unsigned whole = wide && d >= VEC ? d - VEC + 1 : 0;
-#pragma unroll
-        for (int u = 0; u < E / VEC; ++u) {
-            const int c = c0 + u * g * VEC;
-            if ((unsigned)c < whole) {
-                p[u].load(row + c);
-            } else {
-                p[u] = {};
-                if (c < d && c + VEC > 0) {
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j)
-                        if ((unsigned)(c + j) < (unsigned)d) p[u].raw(j, row[c + j]);
-                }
-            }
-        }
+    // whether the window at column c lies in the row, or at least a part of it does
+    static __device__ __forceinline__ bool whole(int c, int d) {
+        return M == kFull || (M == kWhole ? c < d : c >= 0 && c + VEC <= d);
     }
-    __device__ __forceinline__ void get(float (&f)[E]) const {
-#pragma unroll
-        for (int u = 0; u < E / VEC; ++u) {
-            float v[VEC];
-            p[u].get(v);
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) f[u * VEC + j] = v[j];
-        }
+    static __device__ __forceinline__ bool any(int c, int d) {
+        return M == kFull || (M == kWhole ? c < d : c < d && c + VEC > 0);
     }
-    static __device__ __forceinline__ void store(T* __restrict__ row, int c0, int g, int d, bool wide, const float (&f)[E]) {
-        const unsigned whole = wide && d >= VEC ? d - VEC + 1 : 0;
+    // a window that is not whole in the row, or not in memory (at: its first entry)
+    static __device__ __forceinline__ Pack<T, VEC> edge(const T* __restrict__ at, int c, int d) {
+        Pack<T, VEC> q = {};
+        if (M == kShifted) {
 #pragma unroll
-        for (int u = 0; u < E / VEC; ++u) {
-            const int c = c0 + u * g * VEC;
-            if (c >= d) break;
-            float v[VEC];
+            for (int j = 0; j < VEC; ++j)
+                if ((unsigned)(c + j) < (unsigned)d) q.raw(j, at[j]);
+        }
+        return q;
+    }
+    // wide: windows are whole 16-byte words of this row's memory too
+    static __device__ __forceinline__ void store(T* __restrict__ at, int c, int d, bool wide, const float (&f)[VEC]) {
+        Pack<T, VEC> q;
+        q.put(f);
+        if (M != kShifted || (wide && whole(c, d))) {
+            q.store(at);
+        } else {
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) v[j] = f[u * VEC + j];
-            Pack<T, VEC> q;
-            q.put(v);
-            if ((unsigned)c < whole) {
-                q.store(row + c);
-            } else {
-#pragma unroll
-                for (int j = 0; j < VEC; ++j)
-                    if ((unsigned)(c + j) < (unsigned)d) row[c + j] = q.raw(j);
-            }
+            for (int j = 0; j < VEC; ++j)
+                if ((unsigned)(c + j) < (unsigned)d) at[j] = q.raw(j);
         }
     }
 };
 
-constexpr int kMostThreads = 512, kMostParts = 8;
+// A thread's slots in shared memory: OPS operands of NP windows, STAGES times; a warp's lie together.
+template <int NP, int OPS, int STAGES> struct Ring {
+    static constexpr int kStage = OPS * NP * 32;  // 16-byte words of a warp
+    uint4* slots;
+    uint32_t at;
+    int put = 0, got = 0;
+
+    __device__ __forceinline__ Ring(uint4* shared) {
+        slots = shared + (threadIdx.x >> 5) * STAGES * kStage + (threadIdx.x & 31);
+        at = (uint32_t)__cvta_generic_to_shared(slots);
+    }
+    __device__ __forceinline__ void fetch(int op, int u, const void* from) const {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + 16 * (put * kStage + (op * NP + u) * 32)), "l"(from)
+                     : "memory");
+    }
+    __device__ __forceinline__ void sent() {
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        put = put + 1 == STAGES ? 0 : put + 1;
+    }
+    // waits for the oldest stage
+    __device__ __forceinline__ const uint4* next() {
+        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+        const uint4* p = slots + got * kStage;
+        got = got + 1 == STAGES ? 0 : got + 1;
+        return p;
+    }
+    template <typename P> static __device__ __forceinline__ P window(const uint4* stage, int op, int u) {
+        const uint4 w = stage[(op * NP + u) * 32];
+        P q;
+        q.w[0] = w.x, q.w[1] = w.y, q.w[2] = w.z, q.w[3] = w.w;
+        return q;
+    }
+};
+
+// Entries [c, c + N) of a parameter vector of d entries (on 16 bytes unless `loose`); `past` outside it or without one.  Where
+// c is not a multiple of 4 they are cut out of aligned words.
+template <int N, Windows M>
+__device__ __forceinline__ void parameter(const float* __restrict__ v, int c, int d, bool loose, float past, float (&f)[N]) {
+    if (v == nullptr) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) f[j] = past;
+    } else if (M != kShifted) {
+#pragma unroll
+        for (int k = 0; k < N; k += 4) {
+            const float4 q = __ldg(reinterpret_cast<const float4*>(v + c + k));
+            f[k] = q.x, f[k + 1] = q.y, f[k + 2] = q.z, f[k + 3] = q.w;
+        }
+    } else if (!loose && c >= 0 && c + N + 4 <= d) {
+        const int o = c & 3;
+        float w[N + 4];
+#pragma unroll
+        for (int k = 0; k < N + 4; k += 4) {
+            const float4 q = __ldg(reinterpret_cast<const float4*>(v + (c - o) + k));
+            w[k] = q.x, w[k + 1] = q.y, w[k + 2] = q.z, w[k + 3] = q.w;
+        }
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const float lo = o & 1 ? w[j + 1] : w[j], hi = o & 1 ? w[j + 3] : w[j + 2];
+            f[j] = o & 2 ? hi : lo;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) f[j] = (unsigned)(c + j) < (unsigned)d ? v[c + j] : past;
+    }
+}
+
+constexpr int kMostThreads = 512, kMostParts = 8;  // of a block, and blocks of a row
 
 struct RowPlan {
-    int g, rows, parts;  // threads a row and block, rows a block, blocks a row
+    int g, rows, parts;  // threads a row and block, rows a block at a time, blocks a row
+    bool loose;          // weight or bias not on 16 bytes
 };
 
-// Sum over the G threads of a row within a block (the whole warp for G = 32), through `sh`.
-__device__ __forceinline__ float group_sum(float v, float* sh, int g) {
+// Barrier of the G threads of a row in a block (every thread of the block where it has one row).
+__device__ __forceinline__ void group_barrier(const RowPlan& plan, int group) {
+    asm volatile("barrier.sync %0, %1;" ::"r"(group + 1), "r"(plan.g) : "memory");
+}
+
+// Sums of two values over the G threads of a row within a block, through `sh` (one entry a warp, another `sh` in the next
+// call).
+__device__ __forceinline__ float2 group_sum(float2 v, float2* sh, const RowPlan& plan, int group) {
+    v.x = warp_sum(v.x);
+    v.y = warp_sum(v.y);
+    if (plan.g == 32) return v;
+    const int w = plan.g >> 5, lane = threadIdx.x & 31;
+    if (lane == 0) sh[threadIdx.x >> 5] = v;
+    group_barrier(plan, group);
+    v = lane < w ? sh[group * w + lane] : make_float2(0.f, 0.f);
+    return make_float2(warp_sum(v.x), warp_sum(v.y));
+}
+__device__ __forceinline__ float group_sum(float v, float* sh, const RowPlan& plan, int group) {
     v = warp_sum(v);
-    if (g == 32) return v;
-    const int w = g >> 5, warp = threadIdx.x >> 5;
-    if ((threadIdx.x & 31) == 0) sh[warp] = v;
-    __syncthreads();
-    float t = 0;
-    for (int k = warp / w * w, end = k + w; k < end; ++k) t += sh[k];
-    return t;
+    if (plan.g == 32) return v;
+    const int w = plan.g >> 5, lane = threadIdx.x & 31;
+    if (lane == 0) sh[threadIdx.x >> 5] = v;
+    group_barrier(plan, group);
+    return warp_sum(lane < w ? sh[group * w + lane] : 0.f);
 }
 
 // One value pair of every block of the cluster, in every block; `slots` of [kMostParts], another one in the next call.
@@ -293,168 +364,254 @@ __device__ __forceinline__ void cluster_share(float2* slots, float2 v, int rank,
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-template <typename T, int E>
-__global__ void __launch_bounds__(kMostThreads) norm_line_kernel(const T* __restrict__ x, T* __restrict__ y, NormArgs<float> a,
-                                                                 RowPlan plan) {
-    using L = Line<T, E>;
-    __shared__ float sums[kMostThreads / 32], squares[kMostThreads / 32];
-    __shared__ float2 shares[2][kMostParts];
-    const int g = plan.g, t = threadIdx.x % g, rank = (int)(blockIdx.x % (unsigned)plan.parts);
-    const int share = g * E, d = (int)a.d;
-    if (plan.parts > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-    const int64_t step = (int64_t)(gridDim.x / (unsigned)plan.parts) * plan.rows;
-    int64_t i = (int64_t)(blockIdx.x / (unsigned)plan.parts) * plan.rows + threadIdx.x / g;
-    const int shift = shift_of(x + i * a.sn), c0 = rank * share + t * L::VEC - shift;
-    const bool same = shift_of(y + i * a.gn) == shift;
-    // entries of the row in block k's share
-    auto count = [&](int k) { return min(max(d + shift - k * share, 0), share) - (k == 0 ? shift : 0); };
-    float w[E], b[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const int c = L::column(e, c0, g);
-        const bool in = (unsigned)c < (unsigned)d;
-        w[e] = in && a.weight != nullptr ? a.weight[c] : 1.f;
-        b[e] = in && a.bias != nullptr ? a.bias[c] : 0.f;
-    }
-    L next;
-    next.load(x + (i < a.n ? i : 0) * a.sn, c0, g, i < a.n ? d : 0, true);
-    if (plan.parts > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
-    // every thread of a block takes the same turns, also where its row lies past the end
-    for (int64_t top = i - threadIdx.x / g, turn = 0; top < a.n; top += step, i += step, ++turn) {
-        float f[E];
-        next.get(f);
-        const int64_t below = i + step;
-        next.load(x + (below < a.n ? below : 0) * a.sn, c0, g, below < a.n ? d : 0, true);
-        float s = 0;
-#pragma unroll
-        for (int e = 0; e < E; ++e) s += f[e];
-        float mu = group_sum(s, sums, g) / (float)max(count(rank), 1);
-        float q = 0;
-#pragma unroll
-        for (int u = 0; u < E / L::VEC; ++u) {
-            const int c = c0 + u * g * L::VEC;
-            const bool whole = c >= 0 && c + L::VEC <= d;
-#pragma unroll
-            for (int j = 0; j < L::VEC; ++j) {
-                const float v = f[u * L::VEC + j] - mu;
-                if (whole || (unsigned)(c + j) < (unsigned)d) q = fmaf(v, v, q);
-            }
-        }
-        q = group_sum(q, squares, g);
-        if (plan.parts > 1) {
-            float2* slots = shares[turn & 1];
-            cluster_share(slots, make_float2(mu, q), rank, plan.parts);
-            float m = 0;
-            for (int k = 0; k < plan.parts; ++k) m += slots[k].x * ((float)count(k) / (float)d);
-            q = 0;
-            for (int k = 0; k < plan.parts; ++k) {
-                const float c = slots[k].x - m;
-                q += slots[k].y + c * c * (float)count(k);
-            }
-            mu = m;
-        }
-        const float r = 1.f / sqrtf(q / (float)d + a.eps);
-        if (i < a.n) {
-#pragma unroll
-            for (int e = 0; e < E; ++e) f[e] = fmaf((f[e] - mu) * r, w[e], b[e]);
-            L::store(y + i * a.gn, c0, g, d, same, f);
-            if (t == 0 && rank == 0) {
-                if (a.mean != nullptr) a.mean[i] = mu;
-                if (a.rstd != nullptr) a.rstd[i] = r;
-            }
-        }
-    }
+// 1 / sqrt(v): the hardware's estimate and one Newton step.
+__device__ __forceinline__ float inverse_root(float v) {
+    const float r = rsqrtf(v);
+    return v > 0.f && v < INFINITY ? r * fmaf(-0.5f * v * r, r, 1.5f) : r;
 }
 
-// part: [2, gridDim.x / parts * rows, d] sums of gy h and gy over a group's rows (null: not wanted).  gx null: not wanted.
-template <typename T, int E>
-__global__ void __launch_bounds__(kMostThreads) norm_line_grad_kernel(const T* __restrict__ x, const T* __restrict__ gy,
-                                                                      T* __restrict__ gx, NormArgs<float> a, RowPlan plan,
-                                                                      float* __restrict__ part) {
-    using L = Line<T, E>;
-    __shared__ float2 sums[2][kMostThreads / 32];
+template <typename T, int NP, Windows M>
+__global__ void __launch_bounds__(kMostThreads, 2)
+    norm_line_kernel(const T* __restrict__ x, T* __restrict__ y, NormArgs<float> a, RowPlan plan) {
+    using L = Line<T, NP, M>;
+    using P = Pack<T, L::VEC>;
+    constexpr int VEC = L::VEC;
+    extern __shared__ uint4 shared[];
+    __shared__ float sums[kMostThreads / 32], squares[kMostThreads / 32];
     __shared__ float2 shares[2][kMostParts];
-    const int g = plan.g, t = threadIdx.x % g, rank = (int)(blockIdx.x % (unsigned)plan.parts), d = (int)a.d;
+    const int g = plan.g, group = threadIdx.x / g, t = threadIdx.x - group * g;
+    const int rank = (int)(blockIdx.x % (unsigned)plan.parts), share = g * NP * VEC, d = (int)a.d;
     if (plan.parts > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     const int64_t step = (int64_t)(gridDim.x / (unsigned)plan.parts) * plan.rows;
-    const int64_t group = (int64_t)(blockIdx.x / (unsigned)plan.parts) * plan.rows + threadIdx.x / g;
-    int64_t i = group;
-    const int shift = shift_of(x + i * a.sn), c0 = (rank * g * (E / L::VEC) + t) * L::VEC - shift;
-    const bool wide = shift_of(gy + i * a.gn) == shift, same = gx != nullptr && shift_of(gx + i * a.on) == shift;
-    float w[E], gw[E] = {}, gb[E] = {};
+    int64_t i = (int64_t)(blockIdx.x / (unsigned)plan.parts) * plan.rows + group;
+    const int shift = M == kShifted ? shift_of(x + i * a.sn) : 0;
+    const int c0 = rank * share + ((t >> 5) * NP * 32 + (t & 31)) * VEC - shift;
+    const bool same = M != kShifted || shift_of(y + i * a.gn) == shift;
+    // entries of the row in block k's share
+    auto count = [&](int k) { return min(max(d + shift - k * share, 0), share) - (k == 0 ? shift : 0); };
+    const float per = 1.f / (float)d, mine = plan.parts > 1 ? 1.f / (float)max(count(rank), 1) : per;
+    int turns = i < a.n ? (int)((a.n - 1 - i) / step) + 1 : 0, left = turns;
+    const T *ahead = x + i * a.sn + c0, *row = ahead;
+    T* out = y + i * a.gn + c0;
+    const int64_t down = step * a.sn, down_out = step * a.gn;
+    Ring<NP, 1, kStages> ring(shared);
+    auto fetch = [&]() {
+        if (left > 0) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const int c = L::column(e, c0, g);
-        w[e] = (unsigned)c < (unsigned)d && a.weight != nullptr ? a.weight[c] : 1.f;
-    }
-    const float per = 1.f / (float)d;
-    L xn, gn;
-    float mun = 0, rn = 0;
-    auto fetch = [&](int64_t k) {
-        const bool in = k < a.n;
-        xn.load(x + (in ? k : 0) * a.sn, c0, g, in ? d : 0, true);
-        gn.load(gy + (in ? k : 0) * a.gn, c0, g, in ? d : 0, wide);
-        mun = in ? a.mean[k] : 0.f;
-        rn = in ? a.rstd[k] : 0.f;
+            for (int u = 0; u < NP; ++u)
+                if (L::whole(c0 + u * L::STEP, d)) ring.fetch(0, u, ahead + u * L::STEP);
+        }
+        ring.sent();
+        ahead += down;
+        --left;
     };
-    fetch(i);
+#pragma unroll
+    for (int k = 0; k + 1 < kStages; ++k) fetch();
     if (plan.parts > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
-    for (int64_t top = i - threadIdx.x / g, turn = 0; top < a.n; top += step, i += step, ++turn) {
-        float h[E], f[E];
-        xn.get(h);
-        gn.get(f);
-        const float mu = mun, r = rn;
-        fetch(i + step);
-        float s1 = 0, s2 = 0;
+    for (; turns > 0; --turns, i += step, row += down, out += down_out) {
+        // the stage that is filled now was read for the last time in the turn before, and its values have been used
+        fetch();
+        const uint4* stage = ring.next();
+        P p[NP];
+        float s[2] = {};
 #pragma unroll
-        for (int e = 0; e < E; ++e) {  // entries past the row have f = 0
-            h[e] = (h[e] - mu) * r;
-            gw[e] = fmaf(f[e], h[e], gw[e]);
-            gb[e] += f[e];
-            f[e] *= w[e];
-            s1 += f[e];
-            s2 = fmaf(f[e], h[e], s2);
+        for (int u = 0; u < NP; ++u) {
+            const int c = c0 + u * L::STEP;
+            p[u] = L::whole(c, d) ? ring.template window<P>(stage, 0, u) : L::edge(row + u * L::STEP, c, d);
+            float f[VEC];
+            p[u].get(f);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) s[j & 1] += f[j];
         }
-        if (gx == nullptr) continue;  // the same for every thread
-        s1 = warp_sum(s1);
-        s2 = warp_sum(s2);
-        if (g > 32) {
-            const int nw = g >> 5, warp = threadIdx.x >> 5;
-            float2* at = sums[turn & 1];
-            if ((threadIdx.x & 31) == 0) at[warp] = make_float2(s1, s2);
-            __syncthreads();
-            s1 = s2 = 0;
-            for (int k = warp / nw * nw, end = k + nw; k < end; ++k) {
-                s1 += at[k].x;
-                s2 += at[k].y;
+        float mu = group_sum(s[0] + s[1], sums, plan, group) * mine;
+        float q[2] = {};
+#pragma unroll
+        for (int u = 0; u < NP; ++u) {
+            const int c = c0 + u * L::STEP;
+            float f[VEC];
+            p[u].get(f);
+            if (L::whole(c, d)) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) q[j & 1] = fmaf(f[j] - mu, f[j] - mu, q[j & 1]);
+            } else if (M == kShifted) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j)
+                    if ((unsigned)(c + j) < (unsigned)d) q[j & 1] = fmaf(f[j] - mu, f[j] - mu, q[j & 1]);
             }
         }
+        float m2 = group_sum(q[0] + q[1], squares, plan, group);
         if (plan.parts > 1) {
-            float2* slots = shares[turn & 1];
-            cluster_share(slots, make_float2(s1, s2), rank, plan.parts);
-            s1 = s2 = 0;
+            float2* slots = shares[turns & 1];
+            cluster_share(slots, make_float2(mu, m2), rank, plan.parts);
+            mu = m2 = 0;
+            for (int k = 0; k < plan.parts; ++k) mu = fmaf(slots[k].x, (float)count(k) * per, mu);
             for (int k = 0; k < plan.parts; ++k) {
-                s1 += slots[k].x;
-                s2 += slots[k].y;
+                const float c = slots[k].x - mu;
+                m2 += fmaf(c * c, (float)count(k), slots[k].y);
             }
         }
-        s1 *= per;
-        s2 *= per;
-        if (i < a.n) {
+        const float r = inverse_root(fmaf(m2, per, a.eps));
+        if (t == 0 && rank == 0) {
+            if (a.mean != nullptr) a.mean[i] = mu;
+            if (a.rstd != nullptr) a.rstd[i] = r;
+        }
 #pragma unroll
-            for (int e = 0; e < E; ++e) f[e] = r * (f[e] - fmaf(h[e], s2, s1));
-            L::store(gx + i * a.on, c0, g, d, same, f);
+        for (int u = 0; u < NP; ++u) {
+            const int c = c0 + u * L::STEP;
+            if (!L::any(c, d)) continue;
+            float f[VEC], w[VEC], b[VEC];
+            p[u].get(f);
+            parameter<VEC, M>(a.weight, c, d, plan.loose, 1.f, w);
+            parameter<VEC, M>(a.bias, c, d, plan.loose, 0.f, b);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) f[j] = fmaf((f[j] - mu) * r, w[j], b[j]);
+            L::store(out + u * L::STEP, c, d, same, f);
         }
     }
-    if (part == nullptr) return;
-    float* at = part + group * d;
+    asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+// The weight's gradients of a thread's columns stay in its registers all the way down; in the end the groups of a block add
+// theirs up.  part: [2, gridDim.x / parts, d] sums of gy h and of gy (null: not wanted).  gx null: not wanted.
+template <typename T, int NP, Windows M>
+__global__ void __launch_bounds__(kMostThreads, 1) norm_line_grad_kernel(const T* __restrict__ x, const T* __restrict__ gy,
+                                                                         T* __restrict__ gx, NormArgs<float> a, RowPlan plan,
+                                                                         float* __restrict__ part) {
+    using L = Line<T, NP, M>;
+    using P = Pack<T, L::VEC>;
+    constexpr int VEC = L::VEC;
+    extern __shared__ uint4 shared[];  // the ring; in the end [d] floats
+    __shared__ float2 sums[2][kMostThreads / 32];
+    __shared__ float2 shares[2][kMostParts];
+    const int g = plan.g, group = threadIdx.x / g, t = threadIdx.x - group * g;
+    const int rank = (int)(blockIdx.x % (unsigned)plan.parts), share = g * NP * VEC, d = (int)a.d;
+    if (plan.parts > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    const int64_t step = (int64_t)(gridDim.x / (unsigned)plan.parts) * plan.rows;
+    const int64_t i = (int64_t)(blockIdx.x / (unsigned)plan.parts) * plan.rows + group;
+    const int shift = M == kShifted ? shift_of(x + i * a.sn) : 0;
+    const int c0 = rank * share + ((t >> 5) * NP * 32 + (t & 31)) * VEC - shift;
+    const bool wide = M != kShifted || shift_of(gy + i * a.gn) == shift;
+    const bool same = gx != nullptr && (M != kShifted || shift_of(gx + i * a.on) == shift);
+    float gw[NP][VEC] = {}, gb[NP][VEC] = {};
+    const float per = 1.f / (float)d;
+    int turns = i < a.n ? (int)((a.n - 1 - i) / step) + 1 : 0, left = turns;
+    const T *ax = x + i * a.sn + c0, *ag = gy + i * a.gn + c0, *px = ax, *pg = ag;
+    T* out = gx + i * a.on + c0;
+    const float *pm = a.mean + i, *pr = a.rstd + i;
+    const int64_t down_x = step * a.sn, down_g = step * a.gn, down_out = step * a.on;
+    Ring<NP, 2, kStages> ring(shared);
+    auto fetch = [&]() {
+        if (left > 0) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const int c = L::column(e, c0, g);
-        if ((unsigned)c < (unsigned)d) {
-            at[c] = gw[e];
-            at[step * d + c] = gb[e];
+            for (int u = 0; u < NP; ++u)
+                if (L::whole(c0 + u * L::STEP, d)) {
+                    ring.fetch(0, u, ax + u * L::STEP);
+                    if (wide) ring.fetch(1, u, ag + u * L::STEP);
+                }
         }
+        ring.sent();
+        ax += down_x;
+        ag += down_g;
+        --left;
+    };
+#pragma unroll
+    for (int k = 0; k + 1 < kStages; ++k) fetch();
+    if (plan.parts > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    float mun = turns > 0 ? *pm : 0.f, rn = turns > 0 ? *pr : 0.f;
+    for (; turns > 0; --turns, px += down_x, pg += down_g, out += down_out) {
+        const float mu = mun, r = rn;
+        if (turns > 1) {
+            mun = *(pm += step);
+            rn = *(pr += step);
+        }
+        // the stage that is filled now was read for the last time in the turn before, and its values have been used
+        fetch();
+        const uint4* stage = ring.next();
+        auto windows = [&](int u, float(&h)[VEC], float(&f)[VEC]) {
+            const int c = c0 + u * L::STEP;
+            const P p = L::whole(c, d) ? ring.template window<P>(stage, 0, u) : L::edge(px + u * L::STEP, c, d);
+            const P q = L::whole(c, d) && wide ? ring.template window<P>(stage, 1, u) : L::edge(pg + u * L::STEP, c, d);
+            p.get(h);
+            q.get(f);
+        };
+        float s1[2] = {}, s2[2] = {};
+#pragma unroll
+        for (int u = 0; u < NP; ++u) {  // entries past the row have gy = 0
+            const int c = c0 + u * L::STEP;
+            if (!L::any(c, d)) continue;
+            float h[VEC], f[VEC], w[VEC];
+            windows(u, h, f);
+            parameter<VEC, M>(a.weight, c, d, plan.loose, 1.f, w);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                h[j] = (h[j] - mu) * r;
+                gw[u][j] = fmaf(f[j], h[j], gw[u][j]);
+                gb[u][j] += f[j];
+                f[j] *= w[j];
+                s1[j & 1] += f[j];
+                s2[j & 1] = fmaf(f[j], h[j], s2[j & 1]);
+            }
+        }
+        if (gx == nullptr) continue;
+        float2 s = group_sum(make_float2(s1[0] + s1[1], s2[0] + s2[1]), sums[turns & 1], plan, group);
+        if (plan.parts > 1) {
+            float2* slots = shares[turns & 1];
+            cluster_share(slots, s, rank, plan.parts);
+            s = make_float2(0.f, 0.f);
+            for (int k = 0; k < plan.parts; ++k) {
+                s.x += slots[k].x;
+                s.y += slots[k].y;
+            }
+        }
+        s.x *= per;
+        s.y *= per;
+#pragma unroll
+        for (int u = 0; u < NP; ++u) {
+            const int c = c0 + u * L::STEP;
+            if (!L::any(c, d)) continue;
+            float h[VEC], f[VEC], w[VEC];
+            windows(u, h, f);
+            parameter<VEC, M>(a.weight, c, d, plan.loose, 1.f, w);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) f[j] = r * fmaf((h[j] - mu) * r, -s.y, fmaf(f[j], w[j], -s.x));
+            L::store(out + u * L::STEP, c, d, same, f);
+        }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (part == nullptr) return;
+    const int64_t blocks = gridDim.x / (unsigned)plan.parts;
+    float* at = part + (int64_t)(blockIdx.x / (unsigned)plan.parts) * d;
+    if (plan.rows == 1) {
+#pragma unroll
+        for (int u = 0; u < NP; ++u)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                const int c = c0 + u * L::STEP + j;
+                if ((unsigned)c < (unsigned)d) {
+                    at[c] = gw[u][j];
+                    at[blocks * d + c] = gb[u][j];
+                }
+            }
+        return;
+    }
+    // group after group adds its sums, by column: the groups' shifts differ
+    float* fold = reinterpret_cast<float*>(shared);
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        for (int k = 0; k < plan.rows; ++k) {
+            __syncthreads();
+            if (group != k) continue;
+#pragma unroll
+            for (int u = 0; u < NP; ++u)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    const int c = c0 + u * L::STEP + j;
+                    const float v = which == 0 ? gw[u][j] : gb[u][j];
+                    if ((unsigned)c < (unsigned)d) fold[c] = k == 0 ? v : fold[c] + v;
+                }
+        }
+        __syncthreads();
+        for (int c = threadIdx.x; c < d; c += blockDim.x) at[which * blocks * d + c] = fold[c];
     }
 }
 
@@ -483,49 +640,59 @@ __global__ void __launch_bounds__(1024) norm_fold_kernel(const float* __restrict
     if (threadIdx.x == 0 && k < d) out[k] = t;
 }
 
-// The row plan of a width, the entries a thread holds (0: too wide), and the groups of threads that walk the rows.
+// How a width is split; np = 0: too wide.
 struct LinePlan {
     RowPlan plan;
-    int e;
-    int64_t groups;
+    int np;          // windows a thread
+    int64_t blocks;  // of the grid, a cluster counted as one
 };
 
 LinePlan line_plan(int64_t n, int64_t d, int vec, bool shifted, bool backward) {
     LinePlan p{};
-    if (shifted) d += vec - 1;  // room for the furthest shift
-    for (int e = vec; e <= 16; e *= 2)
-        if (d <= 32 * e || e == 16) {
-            p.e = e;
-            break;
-        }
-    int64_t g = ceil_div64(d, (int64_t)p.e * 32) * 32;
+    const int most = 4;
+    const int64_t w = ceil_div64(d + (shifted ? vec - 1 : 0), vec);  // windows, with room for the furthest shift
+    p.np = 1;
+    while (p.np < most && w > 32 * p.np) p.np *= 2;
+    // few rows: more threads a row, as long as they leave the SMs' places empty
+    while (!backward && p.np > 1 && n * ceil_div64(w, p.np) < (int64_t)gpu_sms() * 512) p.np /= 2;
+    int64_t g = ceil_div64(w, 32 * p.np) * 32;
+    while (g > kMostThreads && p.np < most) {
+        p.np *= 2;
+        g = ceil_div64(w, 32 * p.np) * 32;
+    }
     p.plan.parts = 1;
-    while (p.plan.parts < kMostParts && g > kMostThreads) {
+    while (g > kMostThreads && p.plan.parts < kMostParts) {
         p.plan.parts *= 2;
-        g = ceil_div64(d, (int64_t)p.e * 32 * p.plan.parts) * 32;
+        g = ceil_div64(w, (int64_t)32 * p.np * p.plan.parts) * 32;
     }
     if (g > kMostThreads) return {};
     p.plan.g = (int)g;
-    p.plan.rows = g <= 64 ? (int)(128 / g) : 1;
-    // what is resident at once: the kernels take up to 128 registers a thread, the forward ones of few entries 64
-    const int threads = !backward && p.e <= 8 ? 1024 : 512;
-    int64_t blocks = (int64_t)gpu_sms() * (threads / (p.plan.g * p.plan.rows)) / p.plan.parts;
-    const int64_t most = ceil_div64(n, p.plan.rows);
-    blocks = blocks < 1 ? 1 : blocks;
-    // rows of one thread a multiple of a pack's entries apart (see above), where it has more than one
-    if (shifted && blocks < most && blocks % vec != 0) blocks = blocks > vec ? blocks - blocks % vec : vec;
-    p.groups = (blocks < most ? blocks : most) * p.plan.rows;
+    // Blocks that are resident at once: the gradient kernel takes up to 128 registers a thread, the forward one 64; fewer
+    // rows a block rather than fewer blocks
+    const int64_t resident = gpu_sms() * (backward ? 1 : 2) / p.plan.parts, spread = ceil_div64(n, resident);
+    p.plan.rows = (int)(kMostThreads / g < spread ? kMostThreads / g : spread);
+    if (p.plan.parts > 1 || p.plan.rows < 1) p.plan.rows = 1;
+    if (resident * p.plan.rows >= n) {
+        p.blocks = ceil_div64(n, p.plan.rows);
+    } else {
+        // rows of one thread a multiple of a pack's entries apart
+        p.blocks = resident;
+        while (shifted && p.blocks > 1 && p.blocks * p.plan.rows % vec != 0) --p.blocks;
+        if (shifted && p.blocks * p.plan.rows % vec != 0) p.blocks = vec;
+    }
     return p;
 }
 
 template <typename P> struct Same { using type = P; };  // a parameter that is not deduced
 
-template <typename... P> cudaError_t launch_lines(void (*kernel)(P...), const LinePlan& p, cudaStream_t s,
+template <typename... P> cudaError_t launch_lines(void (*kernel)(P...), const LinePlan& p, size_t shared, cudaStream_t s,
                                                   typename Same<P>::type... args) {
+    if (p.blocks * p.plan.parts > 0x7FFFFFFF) return cudaErrorInvalidValue;
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute at[1];
-    cfg.gridDim = dim3((unsigned)(p.groups / p.plan.rows * p.plan.parts));
+    cfg.gridDim = dim3((unsigned)(p.blocks * p.plan.parts));
     cfg.blockDim = dim3((unsigned)(p.plan.g * p.plan.rows));
+    cfg.dynamicSmemBytes = shared;
     cfg.stream = s;
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = (unsigned)p.plan.parts;
@@ -876,6 +1043,29 @@ template <typename T> struct Norm {
         return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (rows <= 1 || ld % VEC == 0);
     }
 
+    template <auto K> struct Kernel { static constexpr auto value = K; };
+
+    // Lets a kernel's blocks take more shared memory than the default allows: once a kernel and device.
+    template <auto K, int BYTES> static cudaError_t allow() {
+        static std::atomic<uint64_t> done[2];  // a bit a device
+        int dev = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e != cudaSuccess) return e;
+        if (dev < 128 && (done[dev / 64] >> (dev % 64) & 1)) return cudaSuccess;
+        e = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES);
+        if (e == cudaSuccess && dev < 128) done[dev / 64] |= uint64_t(1) << (dev % 64);
+        return e;
+    }
+
+    // pick() with the form of the windows
+    template <typename F> static cudaError_t form(const LinePlan& p, int64_t d, bool shifted, F pick) {
+        if (shifted) return pick(std::integral_constant<Windows, kShifted>());
+        if ((int64_t)p.plan.g * p.plan.parts * p.np * VEC == d) return pick(std::integral_constant<Windows, kFull>());
+        return pick(std::integral_constant<Windows, kWhole>());
+    }
+
+    static bool loose(const NormArgs<A>& a) { return !wide(a.weight, 0, 1) || !wide(a.bias, 0, 1); }
+
     static size_t workspace(int64_t n, int64_t d, bool cols, bool backward) {
         if (sizeof(A) != 4 || n == 0) return 0;
         int64_t most = 0;
@@ -886,7 +1076,7 @@ template <typename T> struct Norm {
                 most = need > most ? need : most;
             } else if (backward) {
                 const LinePlan p = line_plan(n, d, VEC, k == 0, true);
-                const int64_t need = p.e != 0 ? 2 * p.groups * d : 0;
+                const int64_t need = p.np != 0 ? 2 * p.blocks * d : 0;
                 most = need > most ? need : most;
             }
         }
@@ -948,10 +1138,23 @@ template <typename T> struct Norm {
                 return w ? forward_strips<VEC>((const T*)x, (T*)y, a, p, (float*)ws, s)
                          : forward_strips<1>((const T*)x, (T*)y, a, p, (float*)ws, s);
             }
-            const LinePlan p = line_plan(a.n, a.d, VEC, !wide(x, a.sn, a.n), false);
-            if (p.e != 0) {
-                auto go = [&](auto kernel) { return launch_lines(kernel, p, s, (const T*)x, (T*)y, a, p.plan); };
-                return p.e == 16 ? go(norm_line_kernel<T, 16>) : p.e == 8 ? go(norm_line_kernel<T, 8>) : go(norm_line_kernel<T, VEC>);
+            const bool shifted = !wide(x, a.sn, a.n) || !wide(y, a.gn, a.n) || a.d % VEC != 0 || loose(a);
+            LinePlan p = line_plan(a.n, a.d, VEC, shifted, false);
+            p.plan.loose = loose(a);
+            if (p.np != 0) {
+                const size_t rows = (size_t)kStages * p.np * 16 * p.plan.g * p.plan.rows;
+                auto go = [&](auto k) {
+                    constexpr auto kernel = decltype(k)::value;
+                    if (const cudaError_t e = allow<kernel, kStages * 4 * 16 * kMostThreads>()) return e;
+                    return launch_lines(kernel, p, rows, s, (const T*)x, (T*)y, a, p.plan);
+                };
+                auto pick = [&](auto mode) {
+                    constexpr Windows M = decltype(mode)::value;
+                    return p.np == 1   ? go(Kernel<norm_line_kernel<T, 1, M>>())
+                           : p.np == 2 ? go(Kernel<norm_line_kernel<T, 2, M>>())
+                                       : go(Kernel<norm_line_kernel<T, 4, M>>());
+                };
+                return form(p, a.d, shifted, pick);
             }
         }
         count_launches(1);
@@ -971,17 +1174,29 @@ template <typename T> struct Norm {
                 return w ? backward_strips<VEC>((const T*)x, (const T*)gy, (T*)gx, gw, gb, a, p, (float*)ws, s)
                          : backward_strips<1>((const T*)x, (const T*)gy, (T*)gx, gw, gb, a, p, (float*)ws, s);
             }
-            const LinePlan p = line_plan(a.n, a.d, VEC, !wide(x, a.sn, a.n), true);
-            if (a.n > 0 && p.e != 0) {
+            const bool shifted = !wide(x, a.sn, a.n) || !wide(gy, a.gn, a.n) || (gx != nullptr && !wide(gx, a.on, a.n)) ||
+                                 a.d % VEC != 0 || loose(a);
+            LinePlan p = line_plan(a.n, a.d, VEC, shifted, true);
+            p.plan.loose = loose(a);
+            if (a.n > 0 && p.np != 0) {
                 float* part = gw != nullptr || gb != nullptr ? (float*)ws : nullptr;
-                auto go = [&](auto kernel) {
-                    return launch_lines(kernel, p, s, (const T*)x, (const T*)gy, (T*)gx, a, p.plan, part);
+                // the rows on their way; in the end, one group's sums (d floats)
+                const size_t rows = (size_t)kStages * 2 * p.np * 16 * p.plan.g * p.plan.rows, sums = (size_t)a.d * 4;
+                const size_t shared = part != nullptr && p.plan.rows > 1 && sums > rows ? sums : rows;
+                auto go = [&](auto k) {
+                    constexpr auto kernel = decltype(k)::value;
+                    if (const cudaError_t e = allow<kernel, kStages * 2 * 4 * 16 * kMostThreads>()) return e;
+                    return launch_lines(kernel, p, shared, s, (const T*)x, (const T*)gy, (T*)gx, a, p.plan, part);
                 };
-                const cudaError_t e = p.e == 16  ? go(norm_line_grad_kernel<T, 16>)
-                                      : p.e == 8 ? go(norm_line_grad_kernel<T, 8>)
-                                                 : go(norm_line_grad_kernel<T, VEC>);
+                auto pick = [&](auto mode) {
+                    constexpr Windows M = decltype(mode)::value;
+                    return p.np == 1   ? go(Kernel<norm_line_grad_kernel<T, 1, M>>())
+                           : p.np == 2 ? go(Kernel<norm_line_grad_kernel<T, 2, M>>())
+                                       : go(Kernel<norm_line_grad_kernel<T, 4, M>>());
+                };
+                const cudaError_t e = form(p, a.d, shifted, pick);
                 if (e != cudaSuccess || part == nullptr) return e;
-                norm_fold_kernel<<<dim3((unsigned)ceil_div64(a.d, 32), 2), dim3(32, 32), 0, s>>>(part, p.groups, a.d, a.d, gw, gb);
+                norm_fold_kernel<<<dim3((unsigned)ceil_div64(a.d, 32), 2), dim3(32, 32), 0, s>>>(part, p.blocks, a.d, a.d, gw, gb);
                 count_launches(1);
                 return cudaGetLastError();
             }
