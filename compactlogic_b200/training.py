@@ -8,16 +8,24 @@
 All four take the layers' own storage (``[batch, features]`` views of feature-major memory) and ordinary row-major tensors
 alike, without copies, and run on the current stream.  A strided tensor that is neither is copied first.
 """
+from functools import lru_cache
 from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
 
 from . import _lib as L
-from .functional import GradSlot, _incoming_grad, _outgoing_grad
+from .functional import GradSlot, _incoming_grad
 
 __all__ = ["LogicDropout", "LogicLayerNorm", "PolicyLoss", "action_log_probs", "dropout", "layer_norm", "policy_loss"]
 
 _LOW = (torch.bfloat16, torch.float16)
+_ACC = {torch.float32: torch.float32, torch.bfloat16: torch.float32, torch.float16: torch.float32,
+        torch.float64: torch.float64}
+_BYTES = {torch.float32: 4, torch.float64: 8}
+
+# The small calls of a training step are bound by the host, so the paths below keep to one allocation where several buffers
+# live and die together, and look up the current stream by its device index.
+_stream = torch._C._cuda_getCurrentRawStream
 
 
 # ------------------------------------------------------------------------------------------------------------ layouts
@@ -39,12 +47,16 @@ def _like(x: torch.Tensor, inner: int) -> torch.Tensor:
     return torch.empty_strided((n, d), (1, n) if inner else (d, 1), dtype=x.dtype, device=x.device)
 
 
-def _on_device(x: torch.Tensor, what: str, **others) -> None:
+def _check(what: str, x: torch.Tensor) -> int:
+    """The dtype code of an input that has to be on a GPU."""
     if not x.is_cuda:
         raise RuntimeError("compactlogic_b200 kernels need CUDA tensors (there is no CPU fallback)")
-    for name, t in others.items():
-        if t is not None and t.device != x.device:
-            raise RuntimeError(f"{what}: {name} is on {t.device}, the input on {x.device}")
+    return L.dtype_code(x.dtype)
+
+
+def _same_device(what: str, x: torch.Tensor, name: str, t: torch.Tensor) -> None:
+    if t.get_device() != x.get_device():
+        raise RuntimeError(f"{what}: {name} is on {t.device}, the input on {x.device}")
 
 
 # ------------------------------------------------------------------------------------------------------------ dropout
@@ -52,9 +64,12 @@ def _drop(x: torch.Tensor, p: float, rescale: bool, seed: int, offset: int, rng:
     x, inner, ld = _matrix(x)
     y = _like(x, inner)
     n, d = x.shape
-    rows, cols = (d, n) if inner else (n, d)
-    L.call("clb_dropout", L.dtype_code(x.dtype), x.data_ptr(), ld, rows, cols, inner, p, rescale, seed, offset, L.ptr(rng),
-           y.data_ptr(), cols, L.stream(x.device))
+    if inner:
+        n, d = d, n
+    status = L.lib().clb_dropout(L.dtype_code(x.dtype), x.data_ptr(), ld, n, d, inner, p, rescale, seed, offset,
+                                 rng.data_ptr() if rng is not None else 0, y.data_ptr(), d, _stream(x.get_device()))
+    if status:
+        L.check(status, "clb_dropout")
     return y
 
 
@@ -80,11 +95,13 @@ class _DropoutFn(torch.autograd.Function):
 def _dropout(x, p, rescale, seed, offset, rng):
     if not 0.0 <= p <= 1.0:
         raise ValueError(f"dropout: p must be in [0, 1], got {p}")
-    _on_device(x, "dropout", rng=rng)
-    L.dtype_code(x.dtype)
+    _check("dropout", x)
+    grad = x.requires_grad and torch.is_grad_enabled()
     if x.dim() == 2:
+        if not grad:
+            return _drop(x, p, rescale, seed, offset, rng)
         # between logic layers with 16-bit activations the gradient is handed over in fp32, past autograd's rounding
-        out_slot = GradSlot() if x.dtype in _LOW and x.requires_grad and torch.is_grad_enabled() else None
+        out_slot = GradSlot() if x.dtype in _LOW else None
         y = _DropoutFn.apply(x, p, rescale, seed, offset, rng, getattr(x, "_clb_slot", None), out_slot)
         if out_slot is not None:
             y._clb_slot = out_slot
@@ -127,9 +144,10 @@ class LogicDropout(torch.nn.Module):
     def forward(self, x):
         if not self.training or self.p == 0.0:
             return x
-        _on_device(x, "LogicDropout", rng_state=self.rng_state)
+        _check("LogicDropout", x)
+        _same_device("LogicDropout", x, "rng_state", self.rng_state)
         used = torch.empty(2, dtype=torch.int64, device=x.device)
-        L.call("clb_dropout_advance", L.ptr(self.rng_state), L.ptr(used), L.stream(x.device))
+        L.call("clb_dropout_advance", self.rng_state.data_ptr(), used.data_ptr(), _stream(x.get_device()))
         return _dropout(x, self.p, self.rescale, 0, 0, used)
 
     def extra_repr(self):
@@ -137,49 +155,65 @@ class LogicDropout(torch.nn.Module):
 
 
 # --------------------------------------------------------------------------------------------------------- layer norm
+@lru_cache(maxsize=256)
+def _norm_bytes(code, n, d, inner, backward):
+    return L.lib().clb_layer_norm_workspace_bytes(code, n, d, inner, backward)
+
+
+def _norm_workspace(code, n, d, inner, backward, device):
+    nbytes = _norm_bytes(code, n, d, inner, backward)
+    return nbytes, torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
 def _norm_forward(x, weight, bias, eps, keep):
-    """(y, x as laid out, its layout, mean, rstd); the last two None without ``keep``."""
+    """(y, x as laid out, statistics [2 n] or None)"""
     x, inner, ld = _matrix(x)
     n, d = x.shape
     y = _like(x, inner)
     code = L.dtype_code(x.dtype)
-    acc = L.acc_dtype(x.dtype)
-    mean, rstd = torch.empty((2, n), dtype=acc, device=x.device).unbind() if keep else (None, None)
-    nbytes = L.lib().clb_layer_norm_workspace_bytes(code, n, d, inner, 0)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
-    L.call("clb_layer_norm_forward", code, x.data_ptr(), ld, n, d, inner, L.ptr(weight), L.ptr(bias), eps, y.data_ptr(),
-           n if inner else d, L.ptr(mean), L.ptr(rstd), L.ptr(ws), nbytes, L.stream(x.device))
-    return y, x, inner, mean, rstd
+    acc = _ACC[x.dtype]
+    stats = torch.empty(2 * n, dtype=acc, device=x.device) if keep else None
+    at = stats.data_ptr() if keep else 0
+    nbytes, ws = _norm_workspace(code, n, d, inner, 0, x.device)
+    status = L.lib().clb_layer_norm_forward(
+        code, x.data_ptr(), ld, n, d, inner, L.ptr(weight), L.ptr(bias), eps, y.data_ptr(), n if inner else d, at,
+        at + n * _BYTES[acc] if keep else 0, L.ptr(ws), nbytes, _stream(x.get_device()))
+    if status:
+        L.check(status, "clb_layer_norm_forward")
+    return y, x, stats
 
 
 class _LayerNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        y, x, ctx.inner, mean, rstd = _norm_forward(x, weight, bias, eps, True)
-        ctx.save_for_backward(x, weight, mean, rstd)
+        y, x, ctx.stats = _norm_forward(x, weight, bias, eps, True)
+        ctx.save_for_backward(x, weight)
         return y
 
     @staticmethod
     def backward(ctx, gy):
-        x, weight, mean, rstd = ctx.saved_tensors
+        x, weight = ctx.saved_tensors
+        stats = ctx.stats
         n, d = x.shape
         x, inner, ld = _matrix(x)
         gy, g_inner, ldg = _matrix(gy)
-        if g_inner != inner and n > 1 and d > 1:
-            gy = gy.t().contiguous().t() if inner else gy.contiguous()
-        if inner:
-            ldg = gy.stride(1) if d > 1 else n
-        else:
-            ldg = gy.stride(0) if n > 1 else d
-        acc = L.acc_dtype(x.dtype)
-        gx = _like(x, inner) if ctx.needs_input_grad[0] else None
-        gw = torch.empty(d, dtype=acc, device=x.device) if ctx.needs_input_grad[1] else None
-        gb = torch.empty(d, dtype=acc, device=x.device) if ctx.needs_input_grad[2] else None
+        if g_inner != inner:
+            if n > 1 and d > 1:
+                gy = gy.t().contiguous().t() if inner else gy.contiguous()
+            ldg = (gy.stride(1) if d > 1 else n) if inner else (gy.stride(0) if n > 1 else d)
+        acc = _ACC[x.dtype]
+        need = ctx.needs_input_grad
+        gx = _like(x, inner) if need[0] else None
+        gw = torch.empty(d, dtype=acc, device=x.device) if need[1] else None
+        gb = torch.empty(d, dtype=acc, device=x.device) if need[2] else None
         code = L.dtype_code(x.dtype)
-        nbytes = L.lib().clb_layer_norm_workspace_bytes(code, n, d, inner, 1)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
-        L.call("clb_layer_norm_backward", code, x.data_ptr(), ld, gy.data_ptr(), ldg, n, d, inner, L.ptr(weight), L.ptr(mean),
-               L.ptr(rstd), L.ptr(gx), n if inner else d, L.ptr(gw), L.ptr(gb), L.ptr(ws), nbytes, L.stream(x.device))
+        nbytes, ws = _norm_workspace(code, n, d, inner, 1, x.device)
+        at = stats.data_ptr()
+        status = L.lib().clb_layer_norm_backward(
+            code, x.data_ptr(), ld, gy.data_ptr(), ldg, n, d, inner, L.ptr(weight), at, at + n * _BYTES[acc], L.ptr(gx),
+            n if inner else d, L.ptr(gw), L.ptr(gb), L.ptr(ws), nbytes, _stream(x.get_device()))
+        if status:
+            L.check(status, "clb_layer_norm_backward")
         return gx, gw, gb, None
 
 
@@ -189,21 +223,23 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
 
     ``weight`` and ``bias`` (optional, [features]) are fp32 for fp32, bf16 and fp16 activations and fp64 for fp64, as the
     layers' parameters are; statistics and the parameters' gradients are summed in that type, in a fixed order."""
-    _on_device(x, "layer_norm", weight=weight, bias=bias)
+    _check("layer_norm", x)
     if x.dim() < 1 or x.shape[-1] < 1:
         raise RuntimeError(f"layer_norm: expected [..., features], got shape {tuple(x.shape)}")
-    acc = L.acc_dtype(x.dtype)
-    L.dtype_code(x.dtype)
+    acc = _ACC[x.dtype]
+    grad = x.requires_grad
     for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None and (t.dtype != acc or t.shape != x.shape[-1:]):
-            raise RuntimeError(f"layer_norm: {name} must be {acc} [{x.shape[-1]}], got {t.dtype} {tuple(t.shape)}")
+        if t is not None:
+            _same_device("layer_norm", x, name, t)
+            if t.dtype != acc or t.shape != x.shape[-1:]:
+                raise RuntimeError(f"layer_norm: {name} must be {acc} [{x.shape[-1]}], got {t.dtype} {tuple(t.shape)}")
+            grad = grad or t.requires_grad
     if not eps >= 0.0:
         raise ValueError(f"layer_norm: eps must not be negative, got {eps}")
     weight = weight if weight is None or weight.is_contiguous() else weight.contiguous()
     bias = bias if bias is None or bias.is_contiguous() else bias.contiguous()
     flat = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    if torch.is_grad_enabled() and (flat.requires_grad or (weight is not None and weight.requires_grad) or
-                                    (bias is not None and bias.requires_grad)):
+    if grad and torch.is_grad_enabled():
         y = _LayerNormFn.apply(flat, weight, bias, eps)
     else:
         y = _norm_forward(flat, weight, bias, eps, False)[0]
@@ -232,63 +268,75 @@ class LogicLayerNorm(torch.nn.Module):
 
 
 # ------------------------------------------------------------------------------------------------------------- losses
+def _per_row(what, name, t, z, lead):
+    """A per-row argument as a contiguous [n] tensor on the logits' device."""
+    if t.get_device() != z.get_device():
+        _same_device(what, z, name, t)
+    if t.shape != lead:
+        raise RuntimeError(f"{what}: {name} must have shape {tuple(lead)}, got {tuple(t.shape)}")
+    return t if t.dim() == 1 and t.is_contiguous() else t.reshape(-1).contiguous()
+
+
 def _rows_of(what, logits, actions, mask):
     """Logits as [n, v] and the per-row arguments flattened to match."""
-    _on_device(logits, what, actions=actions, mask=mask)
-    L.dtype_code(logits.dtype)
+    _check(what, logits)
     lead = logits.shape[:-1]
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise RuntimeError(f"{what}: expected logits [..., classes], got shape {tuple(logits.shape)}")
-    if actions.shape != lead:
-        raise RuntimeError(f"{what}: actions must have shape {tuple(lead)}, got {tuple(actions.shape)}")
     if actions.dtype != torch.int64:
         if actions.is_floating_point() or actions.is_complex() or actions.dtype == torch.bool:
             raise RuntimeError(f"{what}: actions must be integers, got {actions.dtype}")
         actions = actions.long()
+    actions = _per_row(what, "actions", actions, logits, lead)
     if mask is not None:
-        if mask.shape != lead or mask.dtype not in (torch.bool, torch.uint8):
+        if mask.dtype != torch.bool and mask.dtype != torch.uint8:
             raise RuntimeError(f"{what}: mask must be bool {tuple(lead)}, got {mask.dtype} {tuple(mask.shape)}")
-        mask = mask.reshape(-1).contiguous()
+        mask = _per_row(what, "mask", mask, logits, lead)
     z = logits if logits.dim() == 2 else logits.reshape(-1, logits.shape[-1])
-    return z, actions.reshape(-1).contiguous(), mask, lead
+    return z, actions, mask, lead
 
 
 def _logit_grad(z, actions, mask, temperature, stats, slope, scale, upstream, up_stride, gz=None):
-    """gz for one upstream gradient; a given ``gz`` already holds the gradient for an upstream of 1."""
+    """gz for one upstream gradient; a given ``gz`` already holds the gradient for an upstream of 1.  stats, slope and
+    scale are addresses (0: none)."""
     z, inner, ld = _matrix(z)
     n, v = z.shape
     fresh = gz is None
     if fresh:
         gz = _like(z, inner)
-    L.call("clb_logit_grad", L.dtype_code(z.dtype), z.data_ptr(), ld, n, v, inner, actions.data_ptr(), L.ptr(mask),
-           temperature, stats.data_ptr(), L.ptr(slope), L.ptr(scale), L.ptr(upstream), up_stride, not fresh, gz.data_ptr(),
-           n if inner else v, L.stream(z.device))
+    status = L.lib().clb_logit_grad(
+        L.dtype_code(z.dtype), z.data_ptr(), ld, n, v, inner, actions.data_ptr(), L.ptr(mask), temperature, stats, slope, scale,
+        upstream.data_ptr(), up_stride, not fresh, gz.data_ptr(), n if inner else v, _stream(z.get_device()))
+    if status:
+        L.check(status, "clb_logit_grad")
     return gz
 
 
 def _logp_forward(z, actions, mask, temperature, keep):
     z, inner, ld = _matrix(z)
     n, v = z.shape
-    acc = L.acc_dtype(z.dtype)
+    acc = _ACC[z.dtype]
     logp = torch.empty(n, dtype=acc, device=z.device)
     stats = torch.empty(2 * n, dtype=acc, device=z.device) if keep else None
-    L.call("clb_action_logp", L.dtype_code(z.dtype), z.data_ptr(), ld, n, v, inner, actions.data_ptr(), L.ptr(mask),
-           temperature, logp.data_ptr(), L.ptr(stats), L.stream(z.device))
+    status = L.lib().clb_action_logp(L.dtype_code(z.dtype), z.data_ptr(), ld, n, v, inner, actions.data_ptr(), L.ptr(mask),
+                                     temperature, logp.data_ptr(), L.ptr(stats), _stream(z.get_device()))
+    if status:
+        L.check(status, "clb_action_logp")
     return logp, z, stats
 
 
 class _LogProbFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, z, actions, mask, temperature):
-        logp, z, stats = _logp_forward(z, actions, mask, temperature, True)
-        ctx.save_for_backward(z, actions, mask, stats)
+        logp, z, ctx.stats = _logp_forward(z, actions, mask, temperature, True)
+        ctx.save_for_backward(z, actions, mask)
         ctx.temperature = temperature
         return logp
 
     @staticmethod
     def backward(ctx, g):
-        z, actions, mask, stats = ctx.saved_tensors
-        return _logit_grad(z, actions, mask, ctx.temperature, stats, None, None, g, g.stride(0)), None, None, None
+        z, actions, mask = ctx.saved_tensors
+        return (_logit_grad(z, actions, mask, ctx.temperature, ctx.stats.data_ptr(), 0, 0, g, g.stride(0)), None, None, None)
 
 
 def _check_temperature(what, temperature):
@@ -322,40 +370,56 @@ class PolicyLoss(NamedTuple):
     kl: Optional[torch.Tensor]
 
 
+def _policy(z, actions, mask, adv, old, ref, low, high, kl_coef, temperature, reduction, grad):
+    """The loss, the per-row results, the logit gradient (None where it is not made in this pass), and what the gradient of
+    another pass needs: one buffer of slope [n], stats [2 n], scale [1] (and the rows' losses [n])."""
+    z, inner, ld = _matrix(z)
+    n, v = z.shape
+    acc = _ACC[z.dtype]
+    dev = z.device
+    per_row = reduction == "none"
+    logp, ratio = torch.empty(n, dtype=acc, device=dev), torch.empty(n, dtype=acc, device=dev)
+    kl = torch.empty(n, dtype=acc, device=dev) if ref is not None else None
+    loss = torch.empty((n,) if per_row else (), dtype=acc, device=dev)
+    kept = torch.empty(4 * n + 1, dtype=acc, device=dev)
+    at, size = kept.data_ptr(), _BYTES[acc]
+    # the mean's and the sum's gradient is made in the same pass, for an upstream gradient of 1
+    gz = _like(z, inner) if grad and not per_row else None
+    status = L.lib().clb_policy_loss(
+        L.dtype_code(z.dtype), z.data_ptr(), ld, n, v, inner, actions.data_ptr(), L.ptr(mask), adv.data_ptr(), old.data_ptr(),
+        L.ptr(ref), low, high, kl_coef, temperature, reduction == "mean", 0 if per_row else loss.data_ptr(),
+        at + 3 * n * size, loss.data_ptr() if per_row else at + (3 * n + 1) * size, logp.data_ptr(), ratio.data_ptr(),
+        L.ptr(kl), at if grad else 0, at + n * size if grad else 0, L.ptr(gz), n if inner else v, _stream(z.get_device()))
+    if status:
+        L.check(status, "clb_policy_loss")
+    return loss, logp, ratio, kl, z, gz, kept
+
+
 class _PolicyLossFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, z, actions, mask, adv, old, ref, low, high, kl_coef, temperature, reduction, grad):
-        z, inner, ld = _matrix(z)
-        n, v = z.shape
-        acc = L.acc_dtype(z.dtype)
-        dev = z.device
-        logp, ratio, row_loss = (torch.empty(n, dtype=acc, device=dev) for _ in range(3))
-        kl = torch.empty(n, dtype=acc, device=dev) if ref is not None else None
-        slope, stats = torch.empty(3 * n, dtype=acc, device=dev).split((n, 2 * n)) if grad else (None, None)
-        loss, scale = torch.empty((), dtype=acc, device=dev), torch.empty((), dtype=acc, device=dev)
-        # the mean's and the sum's gradient is made in the same pass, for an upstream gradient of 1
-        gz = _like(z, inner) if grad and reduction != "none" else None
-        L.call("clb_policy_loss", L.dtype_code(z.dtype), z.data_ptr(), ld, n, v, inner, actions.data_ptr(), L.ptr(mask),
-               adv.data_ptr(), old.data_ptr(), L.ptr(ref), low, high, kl_coef, temperature, reduction == "mean",
-               loss.data_ptr(), scale.data_ptr(), row_loss.data_ptr(), logp.data_ptr(), ratio.data_ptr(), L.ptr(kl),
-               L.ptr(slope), L.ptr(stats), L.ptr(gz), n if inner else v, L.stream(dev))
-        if grad:
-            ctx.save_for_backward(z, actions, mask, slope, stats, scale)
-            ctx.gz, ctx.temperature = gz, temperature
-            ctx.per_row = reduction == "none"
+    def forward(ctx, z, actions, mask, adv, old, ref, low, high, kl_coef, temperature, reduction):
+        loss, logp, ratio, kl, z, ctx.gz, ctx.kept = _policy(z, actions, mask, adv, old, ref, low, high, kl_coef, temperature,
+                                                             reduction, True)
+        ctx.save_for_backward(z, actions, mask)
+        ctx.temperature, ctx.per_row = temperature, reduction == "none"
         ctx.set_materialize_grads(False)
-        ctx.mark_non_differentiable(*(t for t in (logp, ratio, kl) if t is not None))
-        return row_loss if reduction == "none" else loss, logp, ratio, kl
+        if kl is None:
+            ctx.mark_non_differentiable(logp, ratio)
+        else:
+            ctx.mark_non_differentiable(logp, ratio, kl)
+        return loss, logp, ratio, kl
 
     @staticmethod
     def backward(ctx, g, *unused):
         if g is None:
-            return (None,) * 12
-        z, actions, mask, slope, stats, scale = ctx.saved_tensors
+            return (None,) * 11
+        z, actions, mask = ctx.saved_tensors
+        at, size, n = ctx.kept.data_ptr(), ctx.kept.element_size(), z.shape[0]
         # The gradient made in the forward pass is handed out once; a later call (a retained graph) makes another.
         gz, ctx.gz = ctx.gz, None
-        gz = _logit_grad(z, actions, mask, ctx.temperature, stats, slope, scale, g, g.stride(0) if ctx.per_row else 0, gz)
-        return (gz,) + (None,) * 11
+        gz = _logit_grad(z, actions, mask, ctx.temperature, at + n * size, at, at + 3 * n * size, g,
+                         g.stride(0) if ctx.per_row else 0, gz)
+        return (gz,) + (None,) * 10
 
 
 def policy_loss(logits: torch.Tensor, actions: torch.Tensor, advantages: torch.Tensor, old_log_probs: torch.Tensor, *,
@@ -381,17 +445,18 @@ def policy_loss(logits: torch.Tensor, actions: torch.Tensor, advantages: torch.T
     low, high = clip if isinstance(clip, (tuple, list)) else (clip, clip)
     if not (low >= 0.0 and high >= 0.0):
         raise ValueError(f"policy_loss: clip must not be negative, got {clip}")
-    acc = L.acc_dtype(z.dtype)
+    acc = _ACC[z.dtype]
     given = []
     for name, t in (("advantages", advantages), ("old_log_probs", old_log_probs), ("ref_log_probs", ref_log_probs)):
         if t is not None:
-            _on_device(z, "policy_loss", **{name: t})
-            if t.shape != lead:
-                raise RuntimeError(f"policy_loss: {name} must have shape {tuple(lead)}, got {tuple(t.shape)}")
-            t = t.detach().to(acc).reshape(-1).contiguous()
+            t = _per_row("policy_loss", name, t if t.dtype == acc else t.to(acc), z, lead)
         given.append(t)
-    out = _PolicyLossFn.apply(z, act, m, *given, low, high, kl_coef, temperature, reduction,
-                              z.requires_grad and torch.is_grad_enabled())
+    args = (z, act, m, *given, low, high, kl_coef, temperature, reduction)
+    if z.requires_grad and torch.is_grad_enabled():
+        out = _PolicyLossFn.apply(*args)
+    else:
+        with torch.no_grad():
+            out = _policy(*args, False)[:4]
     if len(lead) != 1:
         out = tuple(t if t is None or (i == 0 and reduction != "none") else t.reshape(lead) for i, t in enumerate(out))
     return PolicyLoss(*out)
