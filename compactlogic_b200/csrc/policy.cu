@@ -526,6 +526,88 @@ __global__ void __launch_bounds__(512) cols_kernel(const T* __restrict__ z, T* _
     }
 }
 
+// Few rows of few classes (decisions out of a group sum): the whole loss in one launch, which is what such a call costs.  One
+// cluster, a thread per row with its logits in registers; the blocks add up the counted rows, then the rows' losses, through
+// distributed shared memory, in a fixed order.
+constexpr int kFewClasses = 16, kFewThreads = 256, kFewRows = 8 * kFewThreads * 4;
+
+template <typename A> __device__ A cluster_sum(A v, A* warps, A* slots, int rank, int parts) {
+    v = warp_sum(v);
+    if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = 0;
+    for (int k = 0; k < kFewThreads / 32; ++k) v += warps[k];
+    if (parts == 1) return v;
+    if (threadIdx.x < parts) {
+        uint32_t local = (uint32_t)__cvta_generic_to_shared(slots + rank), remote;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(threadIdx.x));
+        if constexpr (sizeof(A) == 4)
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote), "f"((float)v) : "memory");
+        else
+            asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(remote), "d"((double)v) : "memory");
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    v = 0;
+    for (int k = 0; k < parts; ++k) v += slots[k];
+    return v;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kFewThreads) few_kernel(const T* __restrict__ z, T* __restrict__ gz,
+                                                          RowArgs<typename Acc<T>::type> a, int parts, int mean,
+                                                          typename Acc<T>::type* loss, typename Acc<T>::type* scale) {
+    using A = typename Acc<T>::type;
+    __shared__ A warps[2][kFewThreads / 32], slots[2][8];
+    const int rank = (int)blockIdx.x;
+    const int64_t first = (int64_t)rank * kFewThreads + threadIdx.x, step = (int64_t)parts * kFewThreads;
+    if (parts > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    A count = 0;  // exact: at most kFewRows
+    for (int64_t i = first; i < a.n; i += step) count += a.mask == nullptr || a.mask[i] ? (A)1 : (A)0;
+    if (parts > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // every block has started
+    count = cluster_sum(count, warps[0], slots[0], rank, parts);
+    a.fixed = mean ? (A)1 / (count > 0 ? count : (A)1) : (A)1;
+    a.scale = nullptr;
+    A total = 0;
+    for (int64_t i = first; i < a.n; i += step) {
+        const bool live = a.mask == nullptr || a.mask[i];
+        T* out = gz + i * a.gn;
+        if (!live) {
+            skip_row(a, i);
+            if (gz != nullptr)
+                for (int64_t j = 0; j < a.v; ++j) out[j * a.gv] = T(0.f);
+            continue;
+        }
+        const RowIn<A> in = row_in<T>(z, a, i);
+        const T* row = z + i * a.sn;
+        A f[kFewClasses], m = lowest<A>(), s = 0;
+#pragma unroll
+        for (int j = 0; j < kFewClasses; ++j) f[j] = j < a.v ? to_acc(row[j * a.sv]) : lowest<A>();
+#pragma unroll
+        for (int j = 0; j < kFewClasses; ++j) m = f[j] > m ? f[j] : m;
+        const A safe = m == lowest<A>() ? (A)0 : m;
+#pragma unroll
+        for (int j = 0; j < kFewClasses; ++j)
+            if (j < a.v) s += soft_exp((f[j] - safe) * a.factor);
+        const A slope = finish_row(a, in, i, m, s, true);
+        total += a.row_loss[i];
+        if (gz == nullptr) continue;
+        const RowGrad<A> g = row_grad(a, slope, m, s);
+        const int64_t act = a.actions[i];
+#pragma unroll
+        for (int j = 0; j < kFewClasses; ++j)
+            if (j < a.v) {
+                const A e = g.w * soft_exp((f[j] - g.m) * a.factor);
+                out[j * a.gv] = from_acc<T>(j == act ? g.c + e : e);
+            }
+    }
+    total = cluster_sum(total, warps[1], slots[1], rank, parts);
+    if (rank == 0 && threadIdx.x == 0) {
+        scale[0] = a.fixed;
+        if (loss != nullptr) loss[0] = total * a.fixed;
+    }
+}
+
 template <typename A> struct GradArgs {
     int64_t n, v, sn, sv, gn, gv;
     const int64_t* actions;
@@ -805,6 +887,13 @@ template <typename T> struct Logits {
         a.row_loss = (A*)row_loss;
         a.gn = cols ? 1 : ldgz;
         a.gv = cols ? ldgz : 1;
+        if (n > 0 && n <= kFewRows && v <= kFewClasses) {
+            int parts = 1;
+            while (parts < 8 && parts * kFewThreads < n) parts *= 2;
+            count_launches(1);
+            return status(launch(few_kernel<T>, parts, dim3(kFewThreads), parts, s, (const T*)z, (T*)gz, a, parts, mean,
+                                 (A*)loss, (A*)scale));
+        }
         const bool count = mean && mask != nullptr;  // else the scale is known here
         a.fixed = mean ? (A)1 / (A)(n > 0 ? n : 1) : (A)1;
         if (count) {
