@@ -161,23 +161,28 @@ template <> struct Two<__half> {
 };
 
 // Rows contiguous, held in registers as 16-byte windows: window k of row i has the entries VEC k - shift ..., where `shift`
-// is how far the row starts past a 16-byte boundary.  Entries outside the row read as -inf and are not written.  A row held
-// this way is short enough for 32-bit indexes.
-template <typename T, int NV> struct RowPart {
-    static constexpr int VEC = 16 / sizeof(T);
+// is how far the row starts past a 16-byte boundary.  Entries outside the row read as -inf and are not written.  A thread has
+// windows a constant distance STRIDE apart, so that they need no arithmetic of their own.  What is known of the windows picks
+// the kernels' form: each is in the row as a whole (kFull), or may be in part or not at all (kShifted).  A row held this way
+// is short enough for 32-bit indexes.
+enum Windows { kFull, kShifted };
+
+template <typename T, int NV, int STRIDE, Windows M> struct RowPart {
+    static constexpr int VEC = 16 / sizeof(T), STEP = VEC * STRIDE;
     Pack<T, VEC> x[NV];
 
-    // windows first, first + stride, ... of the row at `row`
-    __device__ __forceinline__ void load(const T* __restrict__ row, int shift, int v, int first, int stride) {
+    // c: column of the thread's first window
+    __device__ __forceinline__ void load(const T* __restrict__ row, int c, int v) {
         const unsigned whole = v >= VEC ? v - VEC + 1 : 0;  // windows that start in [0, whole) lie in the row
-        int c = VEC * first - shift;
+        const T* at = row + c;
 #pragma unroll
-        for (int u = 0; u < NV; ++u, c += VEC * stride) {
-            if ((unsigned)c < whole) {
-                x[u].load(row + c);
+        for (int u = 0; u < NV; ++u) {
+            if (M == kFull || (unsigned)(c + u * STEP) < whole) {
+                x[u].load(at + u * STEP);
             } else {
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) x[u].raw(j, (unsigned)(c + j) < (unsigned)v ? row[c + j] : T(-INFINITY));
+                for (int j = 0; j < VEC; ++j)
+                    x[u].raw(j, (unsigned)(c + u * STEP + j) < (unsigned)v ? at[u * STEP + j] : T(-INFINITY));
             }
         }
     }
@@ -224,15 +229,15 @@ template <typename T, int NV> struct RowPart {
         r.s = (s[0] + s[1]) + (s[2] + s[3]);
     }
     // the row's gradient without the chosen action's own term; `same`: out's windows lie as the row's
-    __device__ __forceinline__ void grad(T* __restrict__ out, int shift, bool same, int v, int first, int stride,
-                                         const RowGrad<float>& g, float factor) const {
+    __device__ __forceinline__ void grad(T* __restrict__ out, int c, bool same, int v, const RowGrad<float>& g,
+                                         float factor) const {
         const bool tame = fabsf(g.m) < 1e37f;
         const float mk = g.m * factor;
         const unsigned whole = same && v >= VEC ? v - VEC + 1 : 0;
-        int c = VEC * first - shift;
+        T* at = out + c;
 #pragma unroll
-        for (int u = 0; u < NV; ++u, c += VEC * stride) {
-            if (c >= v) break;
+        for (int u = 0; u < NV; ++u) {
+            if (M != kFull && c + u * STEP >= v) break;
             float f[VEC];
             x[u].get(f);
             if (tame) {
@@ -244,22 +249,22 @@ template <typename T, int NV> struct RowPart {
             }
             Pack<T, VEC> y;
             y.put(f);
-            put(out, c, whole, v, y);
+            put(at + u * STEP, c + u * STEP, whole, v, y);
         }
     }
-    __device__ __forceinline__ static void put(T* __restrict__ out, int c, unsigned whole, int v, const Pack<T, VEC>& y) {
-        if ((unsigned)c < whole) {
-            y.store(out + c);
+    static __device__ __forceinline__ void put(T* __restrict__ at, int c, unsigned whole, int v, const Pack<T, VEC>& y) {
+        if (M == kFull || (unsigned)c < whole) {
+            y.store(at);
         } else {
 #pragma unroll
             for (int j = 0; j < VEC; ++j)
-                if ((unsigned)(c + j) < (unsigned)v) out[c + j] = y.raw(j);
+                if ((unsigned)(c + j) < (unsigned)v) at[j] = y.raw(j);
         }
     }
-    __device__ __forceinline__ static void zero(T* __restrict__ out, int shift, bool same, int v, int first, int stride) {
+    __device__ __forceinline__ static void zero(T* __restrict__ out, int c, bool same, int v) {
         const unsigned whole = same && v >= VEC ? v - VEC + 1 : 0;
         const Pack<T, VEC> y = {};
-        for (int u = 0, c = VEC * first - shift; u < NV; ++u, c += VEC * stride) put(out, c, whole, v, y);
+        for (int u = 0; u < NV; ++u) put(out + c + u * STEP, c + u * STEP, whole, v, y);
     }
 };
 
@@ -281,13 +286,14 @@ __global__ void __launch_bounds__(128) rows_group_kernel(const T* __restrict__ z
     const int64_t i = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / G;
     const bool in = i < a.n, live = in && (a.mask == nullptr || a.mask[i]);
     const T* row = z + (in ? i : 0) * a.sn;
-    const int shift = shift_of(row);
-    RowPart<T, NV> part;
+    using Part = RowPart<T, NV, G, kShifted>;
+    const int shift = shift_of(row), c = Part::VEC * lane - shift;
+    Part part;
     Run<float> r;
     RowIn<float> given{};
     if (live) {
         if (lane == 0) given = row_in<T>(z, a, i);
-        part.load(row, shift, v, lane, G);
+        part.load(row, c, v);
         part.sum(r, a.factor);
     }
     warp_merge<G>(r, a.factor);
@@ -304,41 +310,42 @@ __global__ void __launch_bounds__(128) rows_group_kernel(const T* __restrict__ z
     T* out = gz + i * a.gn;
     const bool same = shift_of(out) == shift;
     if (!live) {
-        RowPart<T, NV>::zero(out, shift, same, v, lane, G);
+        Part::zero(out, c, same, v);
         return;
     }
     const RowGrad<float> g = row_grad(a, slope, r.m, r.s);
-    part.grad(out, shift, same, v, lane, G, g, a.factor);
+    part.grad(out, c, same, v, g, a.factor);
     const int64_t act = a.actions[i];
-    if (act >= 0 && act < v && ((int)act + shift) / RowPart<T, NV>::VEC % G == lane) put_action(out, row, act, g, a.factor);
+    if (act >= 0 && act < v && ((int)act + shift) / Part::VEC % G == lane) put_action(out, row, act, g, a.factor);
 }
 
 // Longer rows: a cluster of `parts` blocks per row (one block for parts = 1), NV windows a thread.  The blocks give each
 // other their warps' maxima and sums through distributed shared memory, and every block finishes the row by itself.
-template <typename T, int NV>
+template <typename T, int NV, Windows M>
 __global__ void __launch_bounds__(512, 2) rows_block_kernel(const T* __restrict__ z, T* __restrict__ gz, RowArgs<float> a,
                                                             int parts) {
-    constexpr int VEC = RowPart<T, NV>::VEC;
+    using Part = RowPart<T, NV, 32, M>;
+    constexpr int VEC = Part::VEC;
     __shared__ float2 runs[8 * 16];
     __shared__ RowGrad<float> shared;
     const int64_t i = blockIdx.x / (unsigned)parts;
     const int rank = (int)(blockIdx.x % (unsigned)parts), warps = blockDim.x >> 5, warp = threadIdx.x >> 5,
               lane = threadIdx.x & 31;
     const T* row = z + i * a.sn;
-    const int shift = shift_of(row);
-    const int first = rank * blockDim.x * NV + threadIdx.x, v = (int)a.v;
+    const int shift = M == kFull ? 0 : shift_of(row), v = (int)a.v;
+    const int first = (rank * warps + warp) * 32 * NV + lane, c = VEC * first - shift;  // a warp's windows are neighbours
     T* out = gz != nullptr ? gz + i * a.gn : nullptr;
-    const bool same = gz != nullptr && shift_of(out) == shift;
+    const bool same = gz != nullptr && (M == kFull || shift_of(out) == shift);
     if (a.mask != nullptr && !a.mask[i]) {  // the same in every block of the cluster
         if (rank == 0 && threadIdx.x == 0) skip_row(a, i);
-        if (gz != nullptr) RowPart<T, NV>::zero(out, shift, same, v, first, blockDim.x);
+        if (gz != nullptr) Part::zero(out, c, same, v);
         return;
     }
     if (parts > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // this block has started
     RowIn<float> given{};
     if (threadIdx.x == 0) given = row_in<T>(z, a, i);
-    RowPart<T, NV> part;
-    part.load(row, shift, v, first, blockDim.x);
+    Part part;
+    part.load(row, c, v);
     Run<float> r;
     part.sum(r, a.factor);
     warp_merge(r, a.factor);
@@ -367,11 +374,11 @@ __global__ void __launch_bounds__(512, 2) rows_block_kernel(const T* __restrict_
     if (gz == nullptr) return;
     __syncthreads();
     const RowGrad<float> g = shared;
-    part.grad(out, shift, same, v, first, blockDim.x, g, a.factor);
+    part.grad(out, c, same, v, g, a.factor);
     const int64_t act = a.actions[i];
     if (act >= 0 && act < v) {
-        const int k = ((int)act + shift) / VEC - rank * (int)blockDim.x * NV;
-        if (k >= 0 && k < (int)blockDim.x * NV && k % blockDim.x == threadIdx.x) put_action(out, row, act, g, a.factor);
+        const int k = ((int)act + shift) / VEC;
+        if (k / (32 * NV) == rank * warps + warp && k % 32 == lane) put_action(out, row, act, g, a.factor);
     }
 }
 
@@ -654,32 +661,33 @@ __global__ void __launch_bounds__(256) logit_grad_kernel(const T* __restrict__ z
 }
 
 // The same for contiguous rows, in 16-byte windows: blockDim.y rows a block, `chunks` blocks along a row.
-template <typename T, int NV>
+template <typename T, int NV, int BX, Windows M>
 __global__ void __launch_bounds__(256) rows_grad_kernel(const T* __restrict__ z, T* __restrict__ gz, GradArgs<float> a,
                                                         unsigned chunks) {
     if (a.unless_one && a.upstream[0] == 1.f) return;
-    const int64_t i = (int64_t)(blockIdx.x / chunks) * blockDim.y + threadIdx.y;
+    const int64_t i = (int64_t)(blockIdx.x / chunks) * (256 / BX) + threadIdx.y;
     if (i >= a.n) return;
     const T* row = z + i * a.sn;
     T* out = gz + i * a.gn;
-    const int shift = shift_of(row);
-    const bool same = shift_of(out) == shift;
-    const int first = (int)(blockIdx.x % chunks) * blockDim.x * NV + threadIdx.x, v = (int)a.v;
+    using Part = RowPart<T, NV, BX, M>;
+    const int shift = M == kFull ? 0 : shift_of(row), v = (int)a.v, chunk = (int)(blockIdx.x % chunks);
+    const bool same = M == kFull || shift_of(out) == shift;
+    const int c = Part::VEC * (chunk * BX * NV + (int)threadIdx.x) - shift;
     if (a.mask != nullptr && !a.mask[i]) {
-        RowPart<T, NV>::zero(out, shift, same, v, first, blockDim.x);
+        Part::zero(out, c, same, v);
         return;
     }
-    RowPart<T, NV> part;
-    part.load(row, shift, v, first, blockDim.x);
+    Part part;
+    part.load(row, c, v);
     const int64_t act = a.actions[i];
-    float c = (a.slope != nullptr ? a.slope[i] : 1.f) * (a.scale != nullptr ? a.scale[0] : 1.f) *
+    float k = (a.slope != nullptr ? a.slope[i] : 1.f) * (a.scale != nullptr ? a.scale[0] : 1.f) *
               (a.upstream != nullptr ? a.upstream[i * a.up_stride] : 1.f) * a.inv_t;
-    if (act < 0 || act >= a.v) c = NAN;
-    const RowGrad<float> g = {a.stats[i], c, -c / a.stats[a.n + i]};
-    part.grad(out, shift, same, v, first, blockDim.x, g, a.factor);
+    if (act < 0 || act >= a.v) k = NAN;
+    const RowGrad<float> g = {a.stats[i], k, -k / a.stats[a.n + i]};
+    part.grad(out, c, same, v, g, a.factor);
     if (act >= 0 && act < v) {
-        const int k = ((int)act + shift) / RowPart<T, NV>::VEC - (int)(blockIdx.x % chunks) * (int)blockDim.x * NV;
-        if (k >= 0 && k < (int)blockDim.x * NV && k % blockDim.x == threadIdx.x) put_action(out, row, act, g, a.factor);
+        const int w = ((int)act + shift) / Part::VEC;
+        if (w / (BX * NV) == chunk && w % BX == threadIdx.x) put_action(out, row, act, g, a.factor);
     }
 }
 
@@ -790,12 +798,18 @@ template <typename T> struct Logits {
             if (w <= 64) return group(rows_group_kernel<T, 2, 32>, 32);
             if (w <= 128) return group(rows_group_kernel<T, 4, 32>, 32);
             auto threads = [](int64_t k) { return dim3((unsigned)(ceil_div64(k, 32) * 32)); };
-            if (w <= 4 * kBlockMost) return launch(rows_block_kernel<T, 4>, a.n, threads(ceil_div64(w, 4)), 1, s, z, gz, a, 1);
+            // every window whole: rows on 16 bytes that fill the threads' windows
+            const bool even = aligned && a.v % VEC == 0 &&
+                              (gz == nullptr || (reinterpret_cast<uintptr_t>(gz) % 16 == 0 && (a.n == 1 || a.gn % VEC == 0)));
+            auto block = [&](auto full, auto shifted, int nv, int parts) {
+                const dim3 t = threads(ceil_div64(w, nv * parts));
+                return launch(even && (int64_t)t.x * nv * parts == w ? full : shifted, a.n * parts, t, parts, s, z, gz, a, parts);
+            };
+            if (w <= 4 * kBlockMost) return block(rows_block_kernel<T, 4, kFull>, rows_block_kernel<T, 4, kShifted>, 4, 1);
             for (int most = kBlockMost; most <= 2 * kBlockMost; most *= 2)
                 for (int parts = 1; parts <= 8; parts *= 2)
                     if (w <= (int64_t)parts * 8 * most)
-                        return launch(rows_block_kernel<T, 8>, a.n * parts, threads(ceil_div64(w, 8 * parts)), parts, s, z, gz,
-                                      a, parts);
+                        return block(rows_block_kernel<T, 8, kFull>, rows_block_kernel<T, 8, kShifted>, 8, parts);
         }
         return launch(rows_stream_kernel<T>, a.n, dim3(512), 1, s, z, gz, a);
     }
@@ -808,13 +822,20 @@ template <typename T> struct Logits {
         }
         if constexpr (sizeof(A) == 4) {
             if (a.v < (1 << 30)) {
-            constexpr int NV = 4;
-            const int64_t w = ceil_div64(a.v + 16 / sizeof(T) - 1, 16 / sizeof(T));
-            unsigned bx = 4;
-            while (bx < 256 && bx * NV < w) bx *= 2;
-            const int64_t chunks = ceil_div64(w, bx * NV);
-            return launch(rows_grad_kernel<T, NV>, ceil_div64(a.n, 256 / bx) * chunks, dim3(bx, 256 / bx), 1, s, (const T*)z,
-                          (T*)gz, a, (unsigned)chunks);
+                constexpr int NV = 4, VEC = 16 / sizeof(T);
+                auto even = [&](const void* p, int64_t ld) {
+                    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (a.n == 1 || ld % VEC == 0);
+                };
+                const bool on = even(z, a.sn) && even(gz, a.gn);
+                const int64_t w = ceil_div64(a.v + (on ? 0 : VEC - 1), VEC);
+                auto go = [&](auto full, auto shifted, int bx) {
+                    const int64_t chunks = ceil_div64(w, bx * NV);
+                    return launch(on && a.v == chunks * bx * NV * VEC ? full : shifted, ceil_div64(a.n, 256 / bx) * chunks,
+                                  dim3(bx, 256 / bx), 1, s, (const T*)z, (T*)gz, a, (unsigned)chunks);
+                };
+                if (w <= 8 * NV) return go(rows_grad_kernel<T, NV, 8, kFull>, rows_grad_kernel<T, NV, 8, kShifted>, 8);
+                if (w <= 64 * NV) return go(rows_grad_kernel<T, NV, 64, kFull>, rows_grad_kernel<T, NV, 64, kShifted>, 64);
+                return go(rows_grad_kernel<T, NV, 256, kFull>, rows_grad_kernel<T, NV, 256, kShifted>, 256);
             }
         }
         logit_grad_kernel<T, false><<<blocks(a.n), 256, 0, s>>>((const T*)z, (T*)gz, a);
