@@ -288,13 +288,18 @@ template <int NP, int OPS, int STAGES> struct Ring {
     }
 };
 
-// Entries [c, c + N) of a parameter vector of d entries (on 16 bytes unless `loose`); `past` outside it or without one.  Where
+// Entries [c, c + N) of a parameter vector of d entries (on 16 bytes, or 32 for N = 8, unless `loose`); `past` outside it or without one.  Where
 // c is not a multiple of 4 they are cut out of aligned words.
 template <int N, Windows M>
 __device__ __forceinline__ void parameter(const float* __restrict__ v, int c, int d, bool loose, float past, float (&f)[N]) {
     if (v == nullptr) {
 #pragma unroll
         for (int j = 0; j < N; ++j) f[j] = past;
+    } else if (M != kShifted && N == 8) {
+        // one 32-byte access a lane: two of 16 bytes, 32 apart from lane to lane, take twice the L1 cycles
+        asm("ld.global.nc.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+            : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3]), "=f"(f[4 % N]), "=f"(f[5 % N]), "=f"(f[6 % N]), "=f"(f[7 % N])
+            : "l"(v + c));
     } else if (M != kShifted) {
 #pragma unroll
         for (int k = 0; k < N; k += 4) {
@@ -321,10 +326,16 @@ __device__ __forceinline__ void parameter(const float* __restrict__ v, int c, in
 }
 
 constexpr int kMostThreads = 512, kMostParts = 8;  // of a block, and blocks of a row
+#ifndef GT
+#define GT 640
+#define GN 2
+#endif
+// Threads of the gradient kernel's block, of which an SM has one: 
+template <int NP> constexpr int kGradThreads = NP <= 2 ? GT : 512;
 
 struct RowPlan {
     int g, rows, parts;  // threads a row and block, rows a block at a time, blocks a row
-    bool loose;          // weight or bias not on 16 bytes
+    bool loose;          // weight or bias not on the boundary of a window's entries
 };
 
 // Barrier of the G threads of a row in a block (every thread of the block where it has one row).
@@ -474,14 +485,14 @@ __global__ void __launch_bounds__(kMostThreads, 2)
 // The weight's gradients of a thread's columns stay in its registers all the way down; in the end the groups of a block add
 // theirs up.  part: [2, gridDim.x / parts, d] sums of gy h and of gy (null: not wanted).  gx null: not wanted.
 template <typename T, int NP, Windows M>
-__global__ void __launch_bounds__(kMostThreads, 1) norm_line_grad_kernel(const T* __restrict__ x, const T* __restrict__ gy,
+__global__ void __launch_bounds__(kGradThreads<NP>, 1) norm_line_grad_kernel(const T* __restrict__ x, const T* __restrict__ gy,
                                                                          T* __restrict__ gx, NormArgs<float> a, RowPlan plan,
                                                                          float* __restrict__ part) {
     using L = Line<T, NP, M>;
     using P = Pack<T, L::VEC>;
     constexpr int VEC = L::VEC;
     extern __shared__ uint4 shared[];  // the ring; in the end [d] floats
-    __shared__ float2 sums[2][kMostThreads / 32];
+    __shared__ float2 sums[2][kGradThreads<NP> / 32];
     __shared__ float2 shares[2][kMostParts];
     const int g = plan.g, group = threadIdx.x / g, t = threadIdx.x - group * g;
     const int rank = (int)(blockIdx.x % (unsigned)plan.parts), share = g * NP * VEC, d = (int)a.d;
@@ -649,28 +660,32 @@ struct LinePlan {
 
 LinePlan line_plan(int64_t n, int64_t d, int vec, bool shifted, bool backward) {
     LinePlan p{};
-    const int most = 4;
+    int most = backward ? GN : 4;
+    auto threads = [&](int np) { return !backward ? kMostThreads : np <= 2 ? kGradThreads<1> : kGradThreads<4>; };
+    if (backward && ceil_div64(d + vec, vec) > (int64_t)most * threads(most)) most = 4;
     const int64_t w = ceil_div64(d + (shifted ? vec - 1 : 0), vec);  // windows, with room for the furthest shift
     p.np = 1;
     while (p.np < most && w > 32 * p.np) p.np *= 2;
     // few rows: more threads a row, as long as they leave the SMs' places empty
     while (!backward && p.np > 1 && n * ceil_div64(w, p.np) < (int64_t)gpu_sms() * 512) p.np /= 2;
     int64_t g = ceil_div64(w, 32 * p.np) * 32;
-    while (g > kMostThreads && p.np < most) {
+    while (g > threads(p.np) && p.np < most) {
         p.np *= 2;
         g = ceil_div64(w, 32 * p.np) * 32;
     }
     p.plan.parts = 1;
-    while (g > kMostThreads && p.plan.parts < kMostParts) {
+    while (g > threads(p.np) && p.plan.parts < kMostParts) {
         p.plan.parts *= 2;
         g = ceil_div64(w, (int64_t)32 * p.np * p.plan.parts) * 32;
     }
-    if (g > kMostThreads) return {};
+    if (g > threads(p.np)) return {};
     p.plan.g = (int)g;
     // Blocks that are resident at once: the gradient kernel takes up to 128 registers a thread, the forward one 64; fewer
     // rows a block rather than fewer blocks
-    const int64_t resident = gpu_sms() * (backward ? 1 : 2) / p.plan.parts, spread = ceil_div64(n, resident);
-    p.plan.rows = (int)(kMostThreads / g < spread ? kMostThreads / g : spread);
+    // (clusters: SMs come in groups of 16 or 18, which a cluster does not cross)
+    const int64_t places = p.plan.parts == 1 ? gpu_sms() : gpu_sms() / 18 * (16 / p.plan.parts);
+    const int64_t resident = places * (backward ? 1 : 2), spread = ceil_div64(n, resident);
+    p.plan.rows = (int)(threads(p.np) / g < spread ? threads(p.np) / g : spread);
     if (p.plan.parts > 1 || p.plan.rows < 1) p.plan.rows = 1;
     if (resident * p.plan.rows >= n) {
         p.blocks = ceil_div64(n, p.plan.rows);
@@ -1064,7 +1079,10 @@ template <typename T> struct Norm {
         return pick(std::integral_constant<Windows, kWhole>());
     }
 
-    static bool loose(const NormArgs<A>& a) { return !wide(a.weight, 0, 1) || !wide(a.bias, 0, 1); }
+    // weight or bias off the boundary of a window's entries (16 or 32 bytes)
+    static bool loose(const NormArgs<A>& a) {
+        return (reinterpret_cast<uintptr_t>(a.weight) | reinterpret_cast<uintptr_t>(a.bias)) % (VEC * 4) != 0;
+    }
 
     static size_t workspace(int64_t n, int64_t d, bool cols, bool backward) {
         if (sizeof(A) != 4 || n == 0) return 0;
@@ -1185,7 +1203,7 @@ template <typename T> struct Norm {
                 const size_t shared = part != nullptr && p.plan.rows > 1 && sums > rows ? sums : rows;
                 auto go = [&](auto k) {
                     constexpr auto kernel = decltype(k)::value;
-                    if (const cudaError_t e = allow<kernel, kStages * 2 * 4 * 16 * kMostThreads>()) return e;
+                    if (const cudaError_t e = allow<kernel, kStages * 2 * 4 * 16 * 512>()) return e;
                     return launch_lines(kernel, p, shared, s, (const T*)x, (const T*)gy, (T*)gx, a, p.plan, part);
                 };
                 auto pick = [&](auto mode) {
