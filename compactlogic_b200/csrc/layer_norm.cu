@@ -325,13 +325,13 @@ __device__ __forceinline__ void parameter(const float* __restrict__ v, int c, in
     }
 }
 
-constexpr int kMostThreads = 512, kMostParts = 8;  // of a block, and blocks of a row
-#ifndef GT
-#define GT 640
-#define GN 2
-#endif
-// Threads of the gradient kernel's block, of which an SM has one: 
-template <int NP> constexpr int kGradThreads = NP <= 2 ? GT : 512;
+constexpr int kMostParts = 8;  // blocks of a row
+
+// Threads of a block; the forward kernel has two blocks an SM, the gradient kernel one.  More threads leave each fewer
+// registers: bf16 8192 x 4096 forward takes 29.7 us with 320, 32.8 with 384, 35.4 with 512 (which spills); forward and
+// gradients 96 with 640 threads of two windows, 103 with 512 of four; wider rows need four.
+constexpr int kLineThreads = 320;
+template <int NP> constexpr int kGradThreads = NP <= 2 ? 640 : 512;
 
 struct RowPlan {
     int g, rows, parts;  // threads a row and block, rows a block at a time, blocks a row
@@ -382,13 +382,13 @@ __device__ __forceinline__ float inverse_root(float v) {
 }
 
 template <typename T, int NP, Windows M>
-__global__ void __launch_bounds__(kMostThreads, 2)
+__global__ void __launch_bounds__(kLineThreads, 2)
     norm_line_kernel(const T* __restrict__ x, T* __restrict__ y, NormArgs<float> a, RowPlan plan) {
     using L = Line<T, NP, M>;
     using P = Pack<T, L::VEC>;
     constexpr int VEC = L::VEC;
     extern __shared__ uint4 shared[];
-    __shared__ float sums[kMostThreads / 32], squares[kMostThreads / 32];
+    __shared__ float sums[kLineThreads / 32], squares[kLineThreads / 32];
     __shared__ float2 shares[2][kMostParts];
     const int g = plan.g, group = threadIdx.x / g, t = threadIdx.x - group * g;
     const int rank = (int)(blockIdx.x % (unsigned)plan.parts), share = g * NP * VEC, d = (int)a.d;
@@ -660,10 +660,9 @@ struct LinePlan {
 
 LinePlan line_plan(int64_t n, int64_t d, int vec, bool shifted, bool backward) {
     LinePlan p{};
-    int most = backward ? GN : 4;
-    auto threads = [&](int np) { return !backward ? kMostThreads : np <= 2 ? kGradThreads<1> : kGradThreads<4>; };
-    if (backward && ceil_div64(d + vec, vec) > (int64_t)most * threads(most)) most = 4;
+    auto threads = [&](int np) { return !backward ? kLineThreads : np <= 2 ? kGradThreads<1> : kGradThreads<4>; };
     const int64_t w = ceil_div64(d + (shifted ? vec - 1 : 0), vec);  // windows, with room for the furthest shift
+    const int most = backward && w <= 2 * threads(2) * kMostParts ? 2 : 4;
     p.np = 1;
     while (p.np < most && w > 32 * p.np) p.np *= 2;
     // few rows: more threads a row, as long as they leave the SMs' places empty
@@ -1163,7 +1162,7 @@ template <typename T> struct Norm {
                 const size_t rows = (size_t)kStages * p.np * 16 * p.plan.g * p.plan.rows;
                 auto go = [&](auto k) {
                     constexpr auto kernel = decltype(k)::value;
-                    if (const cudaError_t e = allow<kernel, kStages * 4 * 16 * kMostThreads>()) return e;
+                    if (const cudaError_t e = allow<kernel, kStages * 4 * 16 * kLineThreads>()) return e;
                     return launch_lines(kernel, p, rows, s, (const T*)x, (T*)y, a, p.plan);
                 };
                 auto pick = [&](auto mode) {
