@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(256) norm_rows_grad_kernel(const T* __restrict
     }
 }
 
-// Samples contiguous: a block of 32 x 8 threads per 32 samples, the lanes along the samples.
+// Samples contiguous (fp64): a block of 32 x 8 threads per 32 samples, the lanes along the samples.
 template <typename A> __device__ A column_sum(A v, A (*sh)[33]) {
     __syncthreads();
     sh[threadIdx.y][threadIdx.x] = v;
@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(256) norm_weight_rows_kernel(const T* __restri
     if (gb != nullptr) gb[j] = s2;
 }
 
-// ... and one block per feature when the samples are.
+// ... and one block per feature when the samples are (fp64).
 template <typename T>
 __global__ void __launch_bounds__(256) norm_weight_cols_kernel(const T* __restrict__ x, const T* __restrict__ gy,
                                                                NormArgs<typename Acc<T>::type> a,
@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(kLineThreads, 2)
     for (int k = 0; k + 1 < kStages; ++k) fetch();
     if (plan.parts > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     for (; turns > 0; --turns, i += step, row += down, out += down_out) {
-        // the stage that is filled now was read for the last time in the turn before, and its values have been used
+        __syncwarp();  // the stage that is filled now was read in the turn before
         fetch();
         const uint4* stage = ring.next();
         P p[NP];
@@ -535,7 +535,7 @@ __global__ void __launch_bounds__(kGradThreads<NP>, 1) norm_line_grad_kernel(con
             mun = *(pm += step);
             rn = *(pr += step);
         }
-        // the stage that is filled now was read for the last time in the turn before, and its values have been used
+        __syncwarp();  // the stage that is filled now was read in the turn before
         fetch();
         const uint4* stage = ring.next();
         auto windows = [&](int u, float(&h)[VEC], float(&f)[VEC]) {
@@ -626,29 +626,46 @@ __global__ void __launch_bounds__(kGradThreads<NP>, 1) norm_line_grad_kernel(con
     }
 }
 
-// out[j] = sum over p of part[p * ld + j] for j < d, in a fixed order: 32 columns x 32 shares of the rows a block;
-// blockIdx.y picks the first or the second `groups` rows, and gw or gb.
-__global__ void __launch_bounds__(1024) norm_fold_kernel(const float* __restrict__ part, int64_t groups, int64_t ld, int64_t d,
-                                                         float* gw, float* gb) {
-    __shared__ float sh[32][33];
-    float* out = blockIdx.y == 0 ? gw : gb;
-    if (out == nullptr) return;
-    part += blockIdx.y * groups * ld;
-    const int64_t j = (int64_t)blockIdx.x * 32 + threadIdx.x;
+// Two sums over the same rows: out[k][j] = sum over p < groups of part[(k groups + p) ld + j], j < d, k = 0, 1 (null: not
+// wanted).
+struct Fold {
+    const float* part;
+    int64_t groups, ld, d;
+    float *out0, *out1;
+};
+
+// Up to two of them in one launch, in a fixed order: 32 columns x 8 shares of the rows a block, blockIdx.y picks the sum.
+__global__ void __launch_bounds__(256) norm_fold_kernel(Fold a, Fold b) {
+    __shared__ float sh[8][32];
+    const Fold f = blockIdx.y < 2 ? a : b;
+    const int k = blockIdx.y & 1, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    float* out = k == 0 ? f.out0 : f.out1;
+    const int64_t j = (int64_t)blockIdx.x * 32 + lane;
+    if (out == nullptr || (int64_t)blockIdx.x * 32 >= f.d) return;
+    const float* part = f.part + k * f.groups * f.ld + j;
     float s[4] = {};
-    if (j < d) {
-        int64_t p = threadIdx.y;
-        for (; p + 96 < groups; p += 128) {
+    if (j < f.d) {
+        int64_t p = warp;
+        for (; p + 24 < f.groups; p += 32) {
 #pragma unroll
-            for (int u = 0; u < 4; ++u) s[u] += part[(p + 32 * u) * ld + j];
+            for (int u = 0; u < 4; ++u) s[u] += part[(p + 8 * u) * f.ld];
         }
-        for (; p < groups; p += 32) s[0] += part[p * ld + j];
+        for (; p < f.groups; p += 8) s[0] += part[p * f.ld];
     }
-    sh[threadIdx.y][threadIdx.x] = (s[0] + s[1]) + (s[2] + s[3]);
+    sh[warp][lane] = (s[0] + s[1]) + (s[2] + s[3]);
     __syncthreads();
-    const float t = warp_sum(sh[threadIdx.x][threadIdx.y]);
-    const int64_t k = (int64_t)blockIdx.x * 32 + threadIdx.y;
-    if (threadIdx.x == 0 && k < d) out[k] = t;
+    if (warp != 0 || j >= f.d) return;
+    float t = 0;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) t += sh[w][lane];
+    out[j] = t;
+}
+
+cudaError_t launch_fold(const Fold& a, const Fold& b, cudaStream_t s) {
+    const int64_t d = a.d > b.d ? a.d : b.d;
+    norm_fold_kernel<<<dim3((unsigned)ceil_div64(d, 32), b.part != nullptr ? 4 : 2), 256, 0, s>>>(a, b);
+    count_launches(1);
+    return cudaGetLastError();
 }
 
 // How a width is split; np = 0: too wide.
@@ -859,34 +876,45 @@ __global__ void __launch_bounds__(kColThreads) norm_strip_stats_kernel(const T* 
     }
 }
 
-// mean and rstd from the chunks: 32 samples x 8 shares of the chunks a block
-__global__ void __launch_bounds__(256) norm_strip_fold_kernel(const float* __restrict__ stats, int64_t n, int64_t d,
-                                                              int64_t from, int64_t to, int64_t chunk, int chunks, float eps,
-                                                              float* mean, float* rstd) {
-    __shared__ float sh[8][3][32];
+// mean and rstd from the chunks: 32 samples x 32 shares of the chunks a block, joined pairwise
+__global__ void __launch_bounds__(1024) norm_strip_fold_kernel(const float* __restrict__ stats, int64_t n, int64_t d,
+                                                               int64_t from, int64_t to, int64_t chunk, int chunks, float eps,
+                                                               float* mean, float* rstd) {
+    __shared__ float sh[3][32][33];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t i = from + (int64_t)blockIdx.x * 32 + lane;
     float m = 0, q = 0, n0 = 0;
     if (i < to)
-        for (int k = warp; k < chunks; k += 8) {
+        for (int k = warp; k < chunks; k += 32) {
             const float nk = (float)(d - k * chunk < chunk ? d - k * chunk : chunk), part = nk / (n0 + nk);
             join(m, q, stats[k * n + i], stats[(chunks + k) * n + i], part, n0 * part);
             n0 += nk;
         }
-    sh[warp][0][lane] = m;
-    sh[warp][1][lane] = q;
-    sh[warp][2][lane] = n0;
+    sh[0][warp][lane] = m;
+    sh[1][warp][lane] = q;
+    sh[2][warp][lane] = n0;
     __syncthreads();
-    if (warp != 0 || i >= to) return;
-    for (int k = 1; k < 8; ++k) {
-        const float nk = sh[k][2][lane];
-        if (nk == 0) break;
-        const float part = nk / (n0 + nk);
-        join(m, q, sh[k][0][lane], sh[k][1][lane], part, n0 * part);
-        n0 += nk;
+    // warp w joins the shares of sample w
+    m = sh[0][lane][warp];
+    q = sh[1][lane][warp];
+    n0 = sh[2][lane][warp];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const float m1 = __shfl_xor_sync(0xffffffffu, m, o), q1 = __shfl_xor_sync(0xffffffffu, q, o),
+                    n1 = __shfl_xor_sync(0xffffffffu, n0, o);
+        // both lanes of a pair join in the same order
+        float a = lane & o ? m1 : m, b = lane & o ? q1 : q;
+        const float na = lane & o ? n1 : n0, nb = lane & o ? n0 : n1;
+        const float part = nb > 0.f ? nb / (na + nb) : 0.f;
+        join(a, b, lane & o ? m : m1, lane & o ? q : q1, part, na * part);
+        m = a;
+        q = b;
+        n0 = na + nb;
     }
-    mean[i] = m;
-    rstd[i] = 1.f / sqrtf(q / (float)d + eps);
+    const int64_t at = from + (int64_t)blockIdx.x * 32 + warp;
+    if (lane != 0 || at >= to) return;
+    mean[at] = m;
+    rstd[at] = inverse_root(fmaf(q, 1.f / (float)d, eps));
 }
 
 // y from x, mean and rstd; or gx from x, gy, and the folded sums c1, c2 (GRAD)
@@ -1109,7 +1137,7 @@ template <typename T> struct Norm {
             const int64_t to = from + p.slab < a.n ? from + p.slab : a.n;
             const dim3 grid((unsigned)ceil_div64(to - from, 32 * V), (unsigned)p.chunks);
             norm_strip_stats_kernel<T, V><<<grid, kColThreads, 0, s>>>(x, a, from, to, p.chunk, stats);
-            norm_strip_fold_kernel<<<(unsigned)ceil_div64(to - from, 32), 256, 0, s>>>(stats, a.n, a.d, from, to, p.chunk,
+            norm_strip_fold_kernel<<<(unsigned)ceil_div64(to - from, 32), 1024, 0, s>>>(stats, a.n, a.d, from, to, p.chunk,
                                                                                      p.chunks, a.eps, a.mean, a.rstd);
             norm_strip_apply_kernel<T, V, false><<<grid, kColThreads, 0, s>>>(x, nullptr, y, a, from, to, p.chunk, a.mean,
                                                                               a.rstd, nullptr, nullptr);
@@ -1130,21 +1158,25 @@ template <typename T> struct Norm {
             norm_strip_sums_kernel<T, V><<<grid, kColThreads, 0, s>>>(x, gy, a, from, to, p.chunk, sums,
                                                                       weights ? part : nullptr, from / (32 * V), p.strips);
             count_launches(1);
+            cudaError_t e = cudaGetLastError();
+            if (e != cudaSuccess) return e;
+            // the samples' sums of this slab, and with the last one the parameters' gradients
+            const Fold samples{sums + from, p.chunks, a.n, to - from, c1 + from, c2 + from};
+            const Fold features{part, p.strips, a.d, a.d, gw, gb};
+            const bool last = to == a.n && weights;
+            if (gx != nullptr || last) {
+                e = gx == nullptr ? launch_fold(features, Fold{}, s) : launch_fold(samples, last ? features : Fold{}, s);
+                if (e != cudaSuccess) return e;
+            }
             if (gx != nullptr) {
-                norm_fold_kernel<<<dim3((unsigned)ceil_div64(to - from, 32), 2), dim3(32, 32), 0, s>>>(
-                    sums + from, p.chunks, a.n, to - from, c1 + from, c2 + from);
                 norm_strip_apply_kernel<T, V, true><<<grid, kColThreads, 0, s>>>(x, gy, gx, a, from, to, p.chunk, a.mean,
                                                                                  a.rstd, c1, c2);
-                count_launches(2);
+                count_launches(1);
+                e = cudaGetLastError();
+                if (e != cudaSuccess) return e;
             }
-            const cudaError_t e = cudaGetLastError();
-            if (e != cudaSuccess) return e;
         }
-        if (weights) {
-            norm_fold_kernel<<<dim3((unsigned)ceil_div64(a.d, 32), 2), dim3(32, 32), 0, s>>>(part, p.strips, a.d, a.d, gw, gb);
-            count_launches(1);
-        }
-        return cudaGetLastError();
+        return cudaSuccess;
     }
 
     static cudaError_t forward(const void* x, void* y, const NormArgs<A>& a, bool cols, void* ws, cudaStream_t s) {
@@ -1175,10 +1207,13 @@ template <typename T> struct Norm {
             }
         }
         count_launches(1);
-        if (cols)
-            norm_cols_kernel<T><<<blocks(ceil_div64(a.n, 32)), dim3(32, 8), 0, s>>>((const T*)x, (T*)y, a);
-        else
-            norm_rows_kernel<T><<<blocks(a.n), 256, 0, s>>>((const T*)x, (T*)y, a);
+        if constexpr (sizeof(A) == 8) {
+            if (cols) {
+                norm_cols_kernel<T><<<blocks(ceil_div64(a.n, 32)), dim3(32, 8), 0, s>>>((const T*)x, (T*)y, a);
+                return cudaGetLastError();
+            }
+        }
+        norm_rows_kernel<T><<<blocks(a.n), 256, 0, s>>>((const T*)x, (T*)y, a);
         return cudaGetLastError();
     }
 
@@ -1213,27 +1248,29 @@ template <typename T> struct Norm {
                 };
                 const cudaError_t e = form(p, a.d, shifted, pick);
                 if (e != cudaSuccess || part == nullptr) return e;
-                norm_fold_kernel<<<dim3((unsigned)ceil_div64(a.d, 32), 2), dim3(32, 32), 0, s>>>(part, p.blocks, a.d, a.d, gw, gb);
-                count_launches(1);
+                return launch_fold(Fold{part, p.blocks, a.d, a.d, gw, gb}, Fold{}, s);
+            }
+        }
+        if constexpr (sizeof(A) == 8) {
+            if (cols) {
+                if (gx != nullptr) {
+                    norm_cols_grad_kernel<T><<<blocks(ceil_div64(a.n, 32)), dim3(32, 8), 0, s>>>((const T*)x, (const T*)gy,
+                                                                                               (T*)gx, a);
+                    count_launches(1);
+                }
+                if (gw != nullptr || gb != nullptr) {
+                    norm_weight_cols_kernel<T><<<blocks(a.d), 256, 0, s>>>((const T*)x, (const T*)gy, a, gw, gb);
+                    count_launches(1);
+                }
                 return cudaGetLastError();
             }
         }
         if (gx != nullptr) {
-            if (cols)
-                norm_cols_grad_kernel<T><<<blocks(ceil_div64(a.n, 32)), dim3(32, 8), 0, s>>>((const T*)x, (const T*)gy,
-                                                                                           (T*)gx, a);
-            else
-                norm_rows_grad_kernel<T><<<blocks(a.n), 256, 0, s>>>((const T*)x, (const T*)gy, (T*)gx, a);
+            norm_rows_grad_kernel<T><<<blocks(a.n), 256, 0, s>>>((const T*)x, (const T*)gy, (T*)gx, a);
             count_launches(1);
-            const cudaError_t e = cudaGetLastError();
-            if (e != cudaSuccess) return e;
         }
-        if (gw != nullptr || gb != nullptr) {
-            if (cols)
-                norm_weight_cols_kernel<T><<<blocks(a.d), 256, 0, s>>>((const T*)x, (const T*)gy, a, gw, gb);
-            else
-                norm_weight_rows_kernel<T><<<blocks(ceil_div64(a.d, 32)), dim3(32, 8), 0, s>>>((const T*)x, (const T*)gy, a,
-                                                                                             gw, gb);
+        if (gw != nullptr || gb != nullptr) {  // also of no rows: zeros
+            norm_weight_rows_kernel<T><<<blocks(ceil_div64(a.d, 32)), dim3(32, 8), 0, s>>>((const T*)x, (const T*)gy, a, gw, gb);
             count_launches(1);
         }
         return cudaGetLastError();
