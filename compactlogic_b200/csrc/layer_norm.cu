@@ -296,10 +296,11 @@ __device__ __forceinline__ void parameter(const float* __restrict__ v, int c, in
 #pragma unroll
         for (int j = 0; j < N; ++j) f[j] = past;
     } else if (M != kShifted && N == 8) {
-        // one 32-byte access a lane: two of 16 bytes, 32 apart from lane to lane, take twice the L1 cycles
-        asm("ld.global.nc.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-            : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3]), "=f"(f[4 % N]), "=f"(f[5 % N]), "=f"(f[6 % N]), "=f"(f[7 % N])
-            : "l"(v + c));
+        // One 32-byte access a lane: two of 16 bytes, 32 apart from lane to lane, take twice the L1 cycles.  Volatile: a plain
+        // asm statement is arithmetic to the compiler, which may carry it out before the checks that it stands behind.
+        asm volatile("ld.global.nc.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3]), "=f"(f[4 % N]), "=f"(f[5 % N]), "=f"(f[6 % N]), "=f"(f[7 % N])
+                     : "l"(v + c));
     } else if (M != kShifted) {
 #pragma unroll
         for (int k = 0; k < N; k += 4) {

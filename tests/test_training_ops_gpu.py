@@ -300,6 +300,34 @@ def test_layer_norm_variants(layout):
     assert torch.isnan(y[1]).all() and torch.isnan(y[2]).all() and torch.isfinite(y[[0, 3]]).all()
 
 
+@pytest.mark.parametrize("dtype", LOW)
+@pytest.mark.parametrize("n,d", [(500, 1000), (300, 4096), (7, 96), (40, 2056), (3, 12000), (20, 999)])
+def test_layer_norm_without_parameters(n, d, dtype):
+    """No weight, no bias: nothing is read for them, at any width and form of the windows."""
+    check_norm(n, d, dtype, "rows", affine=False)
+    check_norm(n, d, dtype, "features", affine=False)
+    x = rand((n, d), 1, dtype).requires_grad_()
+    b = rand((d,), 2).requires_grad_()
+    y = cl.layer_norm(x, None, b)  # a bias alone
+    gy = rand((n, d), 3, dtype)
+    _, gb = torch.autograd.grad(y, (x, b), gy)
+    near(gb, gy.double().sum(0), EPS * steps(n) * gy.double().abs().sum(0), torch.float32)
+
+
+def test_layer_norm_parameters_at_odd_places():
+    """Parameters that are slices, off the boundaries of wide reads."""
+    for dtype, d, at in [(torch.bfloat16, 1024, 1), (torch.bfloat16, 1024, 4), (torch.float32, 512, 2), (torch.float16, 1001, 3)]:
+        big = rand((2, d + 8), 5)
+        w, b = big[0, at:at + d], big[1, at:at + d]
+        x, gy = rand((33, d), 6, dtype).requires_grad_(), rand((33, d), 7, dtype)
+        y = cl.layer_norm(x, w, b)
+        gx, = torch.autograd.grad(y, x, gy)
+        want = cl.layer_norm(x, w.clone(), b.clone())
+        gwant, = torch.autograd.grad(want, x, gy)
+        near(y, want.double(), 1e-5, dtype)
+        near(gx, gwant.double(), 1e-5 * float(gwant.double().abs().max()), dtype)
+
+
 def test_layer_norm_shapes_and_refusals():
     for shape in [(0, 5), (7,), (3, 4, 5)]:
         x = rand(shape, 4).requires_grad_()
