@@ -1,7 +1,17 @@
 // Layer norm over the features of [n, d] activations, in either storage layout, forward and backward:
 //   mu_n = mean_d x,  r_n = 1 / sqrt(mean_d (x - mu)^2 + eps),  h = (x - mu) r,  y = h w + b
 //   t = gy w,  gx = r (t - mean_d t - h mean_d (t h)),  gw = sum_n gy h,  gb = sum_n gy
-// Statistics and sums are held in the arithmetic type (fp32; fp64 for fp64 activations).
+// Statistics and sums are held in the arithmetic type (fp32; fp64 for fp64 activations); outputs and gx are rounded once.
+// The variance is a second pass over values that are on the chip, or joined from exact parts (mean, sum of squared
+// differences): no sum of squares about a guessed centre, which one outlying feature would spoil.
+//
+// Forms: rows contiguous, up to 8 blocks of a cluster a row (norm_line_*); samples contiguous (norm_strip_*); wider rows and
+// fp64 (norm_rows_*, norm_cols_*, norm_weight_*), which read their operands up to three times.
+// Measured on a B200 (6.45 TB/s copy rate): bf16 8192 x 4096, forward 37 us (134 MB) and backward 55 us (201 MB and the
+// weight's gradients); fp32 8192 x 4096 forward 56 us (268 MB, 75 %); fp32 16384 features x 512 samples, samples contiguous,
+// both passes 56 us (168 MB at least).  What bounds the rows is the issue of some 15 instructions an entry (forward) and 29
+// (backward) and two block barriers a row; what bounds the strips is that each pass reads its operands twice, and seven
+// launches.
 #include <cuda_runtime.h>
 
 #include <atomic>
@@ -683,7 +693,7 @@ LinePlan line_plan(int64_t n, int64_t d, int vec, bool shifted, bool backward) {
     const int most = backward && w <= 2 * threads(2) * kMostParts ? 2 : 4;
     p.np = 1;
     while (p.np < most && w > 32 * p.np) p.np *= 2;
-    // few rows: more threads a row, as long as they leave the SMs' places empty
+    // few rows: more threads a row, as long as they leave the SMs' places empty (bf16 200 x 4096: 3.5 us, else 3.9)
     while (!backward && p.np > 1 && n * ceil_div64(w, p.np) < (int64_t)gpu_sms() * 512) p.np /= 2;
     int64_t g = ceil_div64(w, 32 * p.np) * 32;
     while (g > threads(p.np) && p.np < most) {
@@ -741,8 +751,8 @@ unsigned blocks(int64_t n) { return (unsigned)(n < (1 << 30) ? n : (1 << 30)); }
 // The statistics run down the strided axis, the weight's gradients along the contiguous one.  First pass: a warp owns a
 // strip of 32 V samples (V a 16-byte pack, or 1 where rows do not start on 16 bytes) and walks down features 8 at a time,
 // all 8 loads in flight; the blocks of `chunk` features leave partial results, which a small kernel folds.  Second pass:
-// elementwise, reading the operands again.  A call runs both passes over one slab of samples after the other, as many as
-// leave a slab's operands in the L2 cache, so that the second pass does not read memory again.
+// elementwise, reading the operands again, out of the L2 cache where they fit.  (Running both passes over one slab of samples
+// after the other, each small enough to stay there, was slower: fp32 64000 x 1024 forward 267 us, in one go 156.)
 
 constexpr int kColThreads = 256, kBatch = 8;
 
@@ -808,16 +818,15 @@ __device__ __forceinline__ void join(float& mean, float& m2, float m, float q, f
     m2 = fmaf(c * c, both, m2 + q);
 }
 
-// stats [2, chunks, n]: mean and sum of squared differences of each chunk's features, for the samples from `from` on.
+// stats [2, chunks, n]: mean and sum of squared differences of each chunk's features.
 template <typename T, int V>
-__global__ void __launch_bounds__(kColThreads) norm_strip_stats_kernel(const T* __restrict__ x, NormArgs<float> a,
-                                                                       int64_t from, int64_t to, int64_t chunk,
+__global__ void __launch_bounds__(kColThreads, 3) norm_strip_stats_kernel(const T* __restrict__ x, NormArgs<float> a, int64_t chunk,
                                                                        float* __restrict__ stats) {
     constexpr int W = kColThreads / 32;
     __shared__ float sh[W][2][32 * V];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t i = from + ((int64_t)blockIdx.x * 32 + lane) * V, j0 = blockIdx.y * chunk;
-    const int left = (int)(to - i < V ? (to > i ? to - i : 0) : V);
+    const int64_t i = ((int64_t)blockIdx.x * 32 + lane) * V, j0 = blockIdx.y * chunk;
+    const int left = (int)(a.n - i < V ? (a.n > i ? a.n - i : 0) : V);
     const int64_t end = j0 + chunk < a.d ? j0 + chunk : a.d;
     float mean[V] = {}, m2[V] = {};
     int64_t n = 0;
@@ -859,7 +868,7 @@ __global__ void __launch_bounds__(kColThreads) norm_strip_stats_kernel(const T* 
     __syncthreads();
     // features warp k has walked over: whole batches from its first on, W batches apart
     for (int c = threadIdx.x; c < 32 * V; c += kColThreads) {
-        const int64_t at = from + (int64_t)blockIdx.x * 32 * V + (c % 32) * V + c / 32;
+        const int64_t at = (int64_t)blockIdx.x * 32 * V + (c % 32) * V + c / 32;
         float m = 0, q = 0;
         int64_t n0 = 0;
         for (int k = 0; k < W; ++k) {
@@ -870,7 +879,7 @@ __global__ void __launch_bounds__(kColThreads) norm_strip_stats_kernel(const T* 
             join(m, q, sh[k][0][c], sh[k][1][c], part, (float)n0 * part);
             n0 += nk;
         }
-        if (at < to) {
+        if (at < a.n) {
             stats[blockIdx.y * a.n + at] = m;
             stats[(gridDim.y + blockIdx.y) * a.n + at] = q;
         }
@@ -879,13 +888,12 @@ __global__ void __launch_bounds__(kColThreads) norm_strip_stats_kernel(const T* 
 
 // mean and rstd from the chunks: 32 samples x 32 shares of the chunks a block, joined pairwise
 __global__ void __launch_bounds__(1024) norm_strip_fold_kernel(const float* __restrict__ stats, int64_t n, int64_t d,
-                                                               int64_t from, int64_t to, int64_t chunk, int chunks, float eps,
-                                                               float* mean, float* rstd) {
+                                                               int64_t chunk, int chunks, float eps, float* mean, float* rstd) {
     __shared__ float sh[3][32][33];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t i = from + (int64_t)blockIdx.x * 32 + lane;
+    const int64_t i = (int64_t)blockIdx.x * 32 + lane;
     float m = 0, q = 0, n0 = 0;
-    if (i < to)
+    if (i < n)
         for (int k = warp; k < chunks; k += 32) {
             const float nk = (float)(d - k * chunk < chunk ? d - k * chunk : chunk), part = nk / (n0 + nk);
             join(m, q, stats[k * n + i], stats[(chunks + k) * n + i], part, n0 * part);
@@ -912,22 +920,22 @@ __global__ void __launch_bounds__(1024) norm_strip_fold_kernel(const float* __re
         q = b;
         n0 = na + nb;
     }
-    const int64_t at = from + (int64_t)blockIdx.x * 32 + warp;
-    if (lane != 0 || at >= to) return;
+    const int64_t at = (int64_t)blockIdx.x * 32 + warp;
+    if (lane != 0 || at >= n) return;
     mean[at] = m;
     rstd[at] = inverse_root(fmaf(q, 1.f / (float)d, eps));
 }
 
 // y from x, mean and rstd; or gx from x, gy, and the folded sums c1, c2 (GRAD)
 template <typename T, int V, bool GRAD>
-__global__ void __launch_bounds__(kColThreads) norm_strip_apply_kernel(const T* __restrict__ x, const T* __restrict__ gy,
-                                                                       T* __restrict__ y, NormArgs<float> a, int64_t from,
-                                                                       int64_t to, int64_t chunk, const float* mean,
-                                                                       const float* rstd, const float* c1, const float* c2) {
-    constexpr int W = kColThreads / 32, B = GRAD ? 4 : 8;
+__global__ void __launch_bounds__(kColThreads, GRAD ? 2 : 3) norm_strip_apply_kernel(const T* __restrict__ x, const T* __restrict__ gy,
+                                                                       T* __restrict__ y, NormArgs<float> a, int64_t chunk,
+                                                                          const float* mean, const float* rstd,
+                                                                          const float* c1, const float* c2) {
+    constexpr int W = kColThreads / 32, B = 4;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t i = from + ((int64_t)blockIdx.x * 32 + lane) * V, j0 = blockIdx.y * chunk;
-    const int left = (int)(to - i < V ? (to > i ? to - i : 0) : V);
+    const int64_t i = ((int64_t)blockIdx.x * 32 + lane) * V, j0 = blockIdx.y * chunk;
+    const int left = (int)(a.n - i < V ? (a.n > i ? a.n - i : 0) : V);
     const int64_t end = j0 + chunk < a.d ? j0 + chunk : a.d, ld = GRAD ? a.od : a.gd;
     if (left == 0) return;
     float mu[V], r[V], k1[V], k2[V];
@@ -974,16 +982,15 @@ __global__ void __launch_bounds__(kColThreads) norm_strip_apply_kernel(const T* 
 // sums [2, chunks, n]: sum of t and of t h over each chunk's features (t = gy w), by sample; and part [2, strips, d]: sums
 // of gy h and of gy over each strip's samples, by feature (null: not wanted).
 template <typename T, int V>
-__global__ void __launch_bounds__(kColThreads) norm_strip_sums_kernel(const T* __restrict__ x, const T* __restrict__ gy,
-                                                                      NormArgs<float> a, int64_t from, int64_t to,
-                                                                      int64_t chunk, float* __restrict__ sums,
-                                                                      float* __restrict__ part, int64_t strip0,
-                                                                      int64_t strips) {
-    constexpr int W = kColThreads / 32, B = kBatch;
+__global__ void __launch_bounds__(kColThreads, 2) norm_strip_sums_kernel(const T* __restrict__ x, const T* __restrict__ gy,
+                                                                      NormArgs<float> a, int64_t chunk,
+                                                                         float* __restrict__ sums,
+                                                                      float* __restrict__ part) {
+    constexpr int W = kColThreads / 32, B = 4;  // 2 B sums over the lanes at once
     __shared__ float sh[W][2][32 * V];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t i = from + ((int64_t)blockIdx.x * 32 + lane) * V, j0 = blockIdx.y * chunk;
-    const int left = (int)(to - i < V ? (to > i ? to - i : 0) : V);
+    const int64_t i = ((int64_t)blockIdx.x * 32 + lane) * V, j0 = blockIdx.y * chunk;
+    const int left = (int)(a.n - i < V ? (a.n > i ? a.n - i : 0) : V);
     const int64_t end = j0 + chunk < a.d ? j0 + chunk : a.d;
     float mu[V], r[V], s1[V] = {}, s2[V] = {};
 #pragma unroll
@@ -1018,7 +1025,7 @@ __global__ void __launch_bounds__(kColThreads) norm_strip_sums_kernel(const T* _
             both[B + u] = q;
         }
         if (part != nullptr) {
-            // 2 B sums over the lanes at once: at each step a lane keeps half of them and hands over the rest
+            // at each step a lane keeps half of its sums and hands over the rest, until one is left
 #pragma unroll
             for (int o = 16, k = B; k >= 1; o >>= 1, k >>= 1) {
                 const bool up = lane & o;
@@ -1028,10 +1035,13 @@ __global__ void __launch_bounds__(kColThreads) norm_strip_sums_kernel(const T* _
                     both[u] = keep + __shfl_xor_sync(0xffffffffu, give, o);
                 }
             }
-            const float total = both[0] + __shfl_xor_sync(0xffffffffu, both[0], 1);
-            const int u = lane >> 1;  // which of the 2 B sums this lane holds
+            constexpr int SAME = 32 / (2 * B);  // neighbouring lanes that hold the same one of the 2 B sums
+            float total = both[0];
+#pragma unroll
+            for (int o = SAME / 2; o >= 1; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+            const int u = lane / SAME;
             const int64_t f = j + (u & (B - 1));
-            if ((lane & 1) == 0 && f < end) part[((u >= B ? strips : 0) + strip0 + blockIdx.x) * a.d + f] = total;
+            if (lane % SAME == 0 && f < end) part[((u >= B ? gridDim.x : 0) + (int64_t)blockIdx.x) * a.d + f] = total;
         }
     }
 #pragma unroll
@@ -1041,13 +1051,13 @@ __global__ void __launch_bounds__(kColThreads) norm_strip_sums_kernel(const T* _
     }
     __syncthreads();
     for (int c = threadIdx.x; c < 32 * V; c += kColThreads) {
-        const int64_t at = from + (int64_t)blockIdx.x * 32 * V + (c % 32) * V + c / 32;
+        const int64_t at = (int64_t)blockIdx.x * 32 * V + (c % 32) * V + c / 32;
         float p = 0, q = 0;
         for (int k = 0; k < W; ++k) {
             p += sh[k][0][c];
             q += sh[k][1][c];
         }
-        if (at < to) {
+        if (at < a.n) {
             sums[blockIdx.y * a.n + at] = p;
             sums[(gridDim.y + blockIdx.y) * a.n + at] = q;
         }
@@ -1055,23 +1065,18 @@ __global__ void __launch_bounds__(kColThreads) norm_strip_sums_kernel(const T* _
 }
 
 struct ColPlan {
-    int v;                 // samples a thread owns
-    int64_t slab, strips;  // samples of a slab (whole strips), strips of the call
-    int64_t chunk;         // features of a block
+    int v;           // samples a thread owns
+    int64_t strips;  // of 32 v samples
+    int64_t chunk;   // features of a block
     int chunks;
 };
 
 ColPlan col_plan(int64_t n, int64_t d, int elem, bool wide, bool backward) {
     ColPlan p{};
     p.v = wide ? 16 / elem : 1;
-    const int64_t strip = 32 * p.v, all = ceil_div64(n, strip);
-    // Half of the L2 cache for a slab's operands; the whole call where it fits
-    const int64_t room = (int64_t)48 << 20, bytes = d * strip * elem * (backward ? 2 : 1);
-    int64_t per = room / bytes < 1 ? 1 : room / bytes;
-    if (all * bytes <= (int64_t)80 << 20 || bytes > room) per = all;
-    p.slab = per * strip;
-    p.strips = all;
-    const int64_t wanted = ceil_div64((int64_t)gpu_sms() * 3, per < all ? per : all), unit = kColThreads / 32 * kBatch;
+    p.strips = ceil_div64(n, 32 * p.v);
+    // as many blocks as are resident at once (or more strips than that)
+    const int64_t resident = (int64_t)gpu_sms() * (backward ? 2 : 3), wanted = resident > p.strips ? resident / p.strips : 1, unit = kColThreads / 32 * kBatch;
     p.chunk = ceil_div64(ceil_div64(d, wanted), unit) * unit;
     p.chunks = (int)ceil_div64(d, p.chunk);
     return p;
@@ -1134,50 +1139,32 @@ template <typename T> struct Norm {
         float* stats = ws + 2 * a.n;
         if (a.mean == nullptr) a.mean = ws;
         if (a.rstd == nullptr) a.rstd = ws + a.n;
-        for (int64_t from = 0; from < a.n; from += p.slab) {
-            const int64_t to = from + p.slab < a.n ? from + p.slab : a.n;
-            const dim3 grid((unsigned)ceil_div64(to - from, 32 * V), (unsigned)p.chunks);
-            norm_strip_stats_kernel<T, V><<<grid, kColThreads, 0, s>>>(x, a, from, to, p.chunk, stats);
-            norm_strip_fold_kernel<<<(unsigned)ceil_div64(to - from, 32), 1024, 0, s>>>(stats, a.n, a.d, from, to, p.chunk,
-                                                                                     p.chunks, a.eps, a.mean, a.rstd);
-            norm_strip_apply_kernel<T, V, false><<<grid, kColThreads, 0, s>>>(x, nullptr, y, a, from, to, p.chunk, a.mean,
-                                                                              a.rstd, nullptr, nullptr);
-            count_launches(3);
-            const cudaError_t e = cudaGetLastError();
-            if (e != cudaSuccess) return e;
-        }
-        return cudaSuccess;
+        const dim3 grid((unsigned)p.strips, (unsigned)p.chunks);
+        norm_strip_stats_kernel<T, V><<<grid, kColThreads, 0, s>>>(x, a, p.chunk, stats);
+        norm_strip_fold_kernel<<<(unsigned)ceil_div64(a.n, 32), 1024, 0, s>>>(stats, a.n, a.d, p.chunk, p.chunks, a.eps, a.mean,
+                                                                           a.rstd);
+        norm_strip_apply_kernel<T, V, false><<<grid, kColThreads, 0, s>>>(x, nullptr, y, a, p.chunk, a.mean, a.rstd, nullptr,
+                                                                          nullptr);
+        count_launches(3);
+        return cudaGetLastError();
     }
 
     template <int V> static cudaError_t backward_strips(const T* x, const T* gy, T* gx, float* gw, float* gb,
                                                         const NormArgs<float>& a, const ColPlan& p, float* ws, cudaStream_t s) {
         float *c1 = ws, *c2 = ws + a.n, *sums = ws + 2 * a.n, *part = sums + 2 * p.chunks * a.n;
         const bool weights = gw != nullptr || gb != nullptr;
-        for (int64_t from = 0; from < a.n; from += p.slab) {
-            const int64_t to = from + p.slab < a.n ? from + p.slab : a.n;
-            const dim3 grid((unsigned)ceil_div64(to - from, 32 * V), (unsigned)p.chunks);
-            norm_strip_sums_kernel<T, V><<<grid, kColThreads, 0, s>>>(x, gy, a, from, to, p.chunk, sums,
-                                                                      weights ? part : nullptr, from / (32 * V), p.strips);
-            count_launches(1);
-            cudaError_t e = cudaGetLastError();
-            if (e != cudaSuccess) return e;
-            // the samples' sums of this slab, and with the last one the parameters' gradients
-            const Fold samples{sums + from, p.chunks, a.n, to - from, c1 + from, c2 + from};
-            const Fold features{part, p.strips, a.d, a.d, gw, gb};
-            const bool last = to == a.n && weights;
-            if (gx != nullptr || last) {
-                e = gx == nullptr ? launch_fold(features, Fold{}, s) : launch_fold(samples, last ? features : Fold{}, s);
-                if (e != cudaSuccess) return e;
-            }
-            if (gx != nullptr) {
-                norm_strip_apply_kernel<T, V, true><<<grid, kColThreads, 0, s>>>(x, gy, gx, a, from, to, p.chunk, a.mean,
-                                                                                 a.rstd, c1, c2);
-                count_launches(1);
-                e = cudaGetLastError();
-                if (e != cudaSuccess) return e;
-            }
-        }
-        return cudaSuccess;
+        const dim3 grid((unsigned)p.strips, (unsigned)p.chunks);
+        norm_strip_sums_kernel<T, V><<<grid, kColThreads, 0, s>>>(x, gy, a, p.chunk, sums, weights ? part : nullptr);
+        count_launches(1);
+        cudaError_t e = cudaGetLastError();
+        if (e != cudaSuccess) return e;
+        const Fold samples{sums, p.chunks, a.n, a.n, c1, c2}, features{part, p.strips, a.d, a.d, gw, gb};
+        if (gx == nullptr) return weights ? launch_fold(features, Fold{}, s) : cudaSuccess;
+        e = launch_fold(samples, weights ? features : Fold{}, s);
+        if (e != cudaSuccess) return e;
+        norm_strip_apply_kernel<T, V, true><<<grid, kColThreads, 0, s>>>(x, gy, gx, a, p.chunk, a.mean, a.rstd, c1, c2);
+        count_launches(1);
+        return cudaGetLastError();
     }
 
     static cudaError_t forward(const void* x, void* y, const NormArgs<A>& a, bool cols, void* ws, cudaStream_t s) {

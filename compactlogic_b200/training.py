@@ -280,6 +280,11 @@ def _per_row(what, name, t, z, lead):
 def _rows_of(what, logits, actions, mask):
     """Logits as [n, v] and the per-row arguments flattened to match."""
     _check(what, logits)
+    if logits.dim() == 2 and actions.dtype is torch.int64 and mask is None:  # the common call, in few steps
+        n, v = logits.shape
+        if v and actions.dim() == 1 and actions.shape[0] == n and actions.is_contiguous() and actions.is_cuda and \
+                actions.get_device() == logits.get_device():
+            return logits, actions, None, (n,)
     lead = logits.shape[:-1]
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise RuntimeError(f"{what}: expected logits [..., classes], got shape {tuple(logits.shape)}")
@@ -447,9 +452,11 @@ def policy_loss(logits: torch.Tensor, actions: torch.Tensor, advantages: torch.T
         raise ValueError(f"policy_loss: clip must not be negative, got {clip}")
     acc = _ACC[z.dtype]
     given = []
+    n, dev = z.shape[0], z.get_device()
     for name, t in (("advantages", advantages), ("old_log_probs", old_log_probs), ("ref_log_probs", ref_log_probs)):
-        if t is not None:
-            t = _per_row("policy_loss", name, t if t.dtype == acc else t.to(acc), z, lead)
+        if t is not None and not (t.dtype is acc and t.dim() == 1 and t.shape[0] == n and len(lead) == 1 and
+                                  t.is_contiguous() and t.get_device() == dev):
+            t = _per_row("policy_loss", name, t if t.dtype is acc else t.to(acc), z, lead)
         given.append(t)
     args = (z, act, m, *given, low, high, kl_coef, temperature, reduction)
     if z.requires_grad and torch.is_grad_enabled():
