@@ -10,7 +10,7 @@
 // Measured on a B200 (6.45 TB/s copy rate): bf16 8192 x 4096, forward 37 us (134 MB) and backward 55 us (201 MB and the
 // weight's gradients); fp32 8192 x 4096 forward 56 us (268 MB, 75 %); fp32 16384 features x 512 samples, samples contiguous,
 // both passes 56 us (168 MB at least).  What bounds the rows is the issue of some 15 instructions an entry (forward) and 29
-// (backward) and two block barriers a row; what bounds the strips is that each pass reads its operands twice, and seven
+// (backward) and two block barriers a row; what bounds the strips is that each pass reads its operands twice, and six
 // launches.
 #include <cuda_runtime.h>
 
