@@ -9,7 +9,8 @@
 //
 // What bounds it: 2 bytes in and 2 out an element of 16 bits stand against ten rounds of two 32 x 32 -> 64 multiplies for
 // four elements, some 15 instructions an element with the conversion and the choice, so integer issue is as near as memory.
-// bf16 64000 x 1024, one pass of 262 MB: 54 us, 4.9 TB/s, 75 % of the card's copy rate.  The first kernel, one counter at a
+// bf16 64000 x 1024, one pass of 262 MB: 54 us, 4.9 TB/s, 75 % of the card's copy rate; fp32 32000 x 1024, as many bytes for half
+// the draws: 47 us, 87 %.  The first kernel, one counter at a
 // time and a block per short piece of a row, issued 32 instructions an element and took 97 us.
 #include <cuda_runtime.h>
 
@@ -30,9 +31,7 @@ template <int N> __device__ __forceinline__ void philox(uint32_t (&c)[4][N], uin
     for (int r = 0; r < 10; ++r) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            uint64_t p0, p1;
-            asm("mul.wide.u32 %0, %1, 0xD2511F53;" : "=l"(p0) : "r"(c[0][i]));
-            asm("mul.wide.u32 %0, %1, 0xCD9E8D57;" : "=l"(p1) : "r"(c[2][i]));
+            const uint64_t p0 = (uint64_t)c[0][i] * 0xD2511F53u, p1 = (uint64_t)c[2][i] * 0xCD9E8D57u;
             c[0][i] = (uint32_t)(p1 >> 32) ^ c[1][i] ^ k0;
             c[1][i] = (uint32_t)p1;
             c[2][i] = (uint32_t)(p0 >> 32) ^ c[3][i] ^ k1;
@@ -51,7 +50,10 @@ struct DropArgs {
     double scale;
 };
 
-constexpr int kThreads = 128, kBlocks = 5;
+// Blocks an SM: the registers of 16-bit elements, twice as many a thread, fit five (bf16 64000 x 1024, both passes: 107 us,
+// with six 113), those of fp32 six (32000 x 1024: 93 us, with five 100).
+constexpr int kThreads = 128;
+template <typename T> constexpr int kBlocks = sizeof(T) == 2 ? 5 : 6;
 
 // The words of NC neighbouring 2 x 2 blocks along the contiguous axis.
 template <int NC, bool BATCH_INNER>
@@ -100,7 +102,7 @@ __device__ __forceinline__ void drop(Pack<T, VEC> (&v)[2], uint32_t inner, uint3
 // loads in flight while it draws the words of the current one.  Rows start on 16 bytes.  BATCH_INNER: the
 // contiguous axis is n (feature-major storage), else d.
 template <typename T, int VEC, bool BATCH_INNER, bool RESCALE>
-__global__ void __launch_bounds__(kThreads, kBlocks) dropout_kernel(const T* __restrict__ x, T* __restrict__ y, DropArgs a) {
+__global__ void __launch_bounds__(kThreads, kBlocks<T>) dropout_kernel(const T* __restrict__ x, T* __restrict__ y, DropArgs a) {
     using A = typename Acc<T>::type;
     const int64_t c = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * VEC;
     if (c >= a.cols) return;
@@ -155,7 +157,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) dropout_kernel(const T* __r
 // thread none); blockDim.x is at most a warp, so no warp waits for another.  gridDim.y * blockDim.y is a multiple of VEC / 2 wherever a thread has a second pair of rows: the shifts of
 // its rows are then the same all the way down.
 template <typename T, bool BATCH_INNER, bool RESCALE>
-__global__ void __launch_bounds__(kThreads, kBlocks) dropout_shifted_kernel(const T* __restrict__ x, T* __restrict__ y,
+__global__ void __launch_bounds__(kThreads, kBlocks<T>) dropout_shifted_kernel(const T* __restrict__ x, T* __restrict__ y,
                                                                             DropArgs a) {
     using A = typename Acc<T>::type;
     constexpr int VEC = 16 / sizeof(T), NC = VEC / 2;
@@ -294,7 +296,7 @@ cudaError_t launch(const T* x, T* y, const DropArgs& a, bool batch_inner, cudaSt
     // As many blocks as are resident at once, each walking down the rows; four times that for shifted rows, whose blocks
     // are rounded to whole shifts and would leave SMs idle (fp16 1001 x 16383, both passes: 75 us with one wave, 51 with
     // four, 57 with eight).
-    int64_t most = (int64_t)gpu_sms() * kBlocks * (wide ? 1 : 4) / gx;
+    int64_t most = (int64_t)gpu_sms() * kBlocks<T> * (wide ? 1 : 4) / gx;
     if (!wide) most -= most % (V / 2);
     if (most < V / 2) most = V / 2;
     const dim3 grid((unsigned)gx, (unsigned)(gy < most ? gy : most));

@@ -17,8 +17,8 @@
 // (rows_group_kernel); long ones by a block or a cluster of up to 8 (rows_block_kernel); samples contiguous (cols_kernel);
 // rows beyond a cluster's registers, and fp64 (rows_stream_kernel), read twice.
 // Measured on a B200 (6.45 TB/s copy rate): bf16 2048 x 131072 with its gradient 242 us (1.07 GB, 4.4 TB/s, 69 %), fp32 1777 x
-// 50001 with a third of the rows masked 147 us (62 %), log-probabilities of bf16 4096 x 32768 with their gradient 141 us (805
-// MB over the two calls, 89 %).  What bounds the long rows: two exponentials an entry (16 a clock and SM: 119 of the 242 us)
+// 50001 with a third of the rows masked 147 us (63 %), log-probabilities of bf16 4096 x 32768 with their gradient 135 us (805
+// MB over the two calls, 93 %).  What bounds the long rows: two exponentials an entry (16 a clock and SM: 119 of the 242 us)
 // among 12 instructions, and the wait of a cluster's blocks for one another between the two halves.  Measured and dropped:
 // clusters that walk over the rows with the next row on its way to shared memory (308 us: fewer clusters fit than blocks),
 // and one block a row that reads the row again out of the L2 cache (242 to 276 us).
@@ -333,12 +333,14 @@ __global__ void __launch_bounds__(128) rows_group_kernel(const T* __restrict__ z
     if (act >= 0 && act < v && ((int)act + shift) / Part::VEC % G == lane) put_action(out, row, act, g, a.factor);
 }
 
-// Longer rows: a cluster of `parts` blocks per row (one block for parts = 1), NV windows a thread.  The blocks give each
+constexpr int kWindows = 8;
+
+// Longer rows: a cluster of `parts` blocks per row (one block for parts = 1), kWindows windows a thread.  The blocks give each
 // other their warps' maxima and sums through distributed shared memory, and every block finishes the row by itself.
-template <typename T, int NV, Windows M>
+template <typename T, Windows M>
 __global__ void __launch_bounds__(512, 2) rows_block_kernel(const T* __restrict__ z, T* __restrict__ gz, RowArgs<float> a,
                                                             int parts) {
-    using Part = RowPart<T, NV, 32, M>;
+    using Part = RowPart<T, kWindows, 32, M>;
     constexpr int VEC = Part::VEC;
     __shared__ float2 runs[8 * 16];
     __shared__ RowGrad<float> shared;
@@ -347,7 +349,7 @@ __global__ void __launch_bounds__(512, 2) rows_block_kernel(const T* __restrict_
               lane = threadIdx.x & 31;
     const T* row = z + i * a.sn;
     const int shift = M == kFull ? 0 : shift_of(row), v = (int)a.v;
-    const int first = (rank * warps + warp) * 32 * NV + lane, c = VEC * first - shift;  // a warp's windows are neighbours
+    const int first = (rank * warps + warp) * 32 * kWindows + lane, c = VEC * first - shift;  // a warp's windows are neighbours
     T* out = gz != nullptr ? gz + i * a.gn : nullptr;
     const bool same = gz != nullptr && (M == kFull || shift_of(out) == shift);
     if (a.mask != nullptr && !a.mask[i]) {  // the same in every block of the cluster
@@ -392,7 +394,7 @@ __global__ void __launch_bounds__(512, 2) rows_block_kernel(const T* __restrict_
     const int64_t act = a.actions[i];
     if (act >= 0 && act < v) {
         const int k = ((int)act + shift) / VEC;
-        if (k / (32 * NV) == rank * warps + warp && k % 32 == lane) put_action(out, row, act, g, a.factor);
+        if (k / (32 * kWindows) == rank * warps + warp && k % 32 == lane) put_action(out, row, act, g, a.factor);
     }
 }
 
@@ -760,8 +762,7 @@ unsigned blocks(int64_t n) { return (unsigned)(n < (1 << 30) ? n : (1 << 30)); }
 
 template <typename P> struct Same { using type = P; };  // a parameter that is not deduced
 
-// Threads of a block of rows_block_kernel; twice as many where eight such blocks do not hold a row.  Blocks of 256 threads
-// hold 32 KB of a row and four of them an SM's registers; with 512 (two an SM) bf16 2048 x 131072 takes 267 us, with 256 262.
+// Threads of a block of rows_block_kernel; twice as many for one block a row, and where eight such blocks do not hold it.
 constexpr int kBlockMost = 256;
 
 template <typename T> struct Logits {
@@ -807,25 +808,32 @@ template <typename T> struct Logits {
             const bool aligned = reinterpret_cast<uintptr_t>(z) % 16 == 0 && (a.n == 1 || a.sn % VEC == 0);
             const int64_t w = ceil_div64(a.v + (aligned ? 0 : VEC - 1), VEC);
             auto group = [&](auto kernel, int g) { return launch(kernel, ceil_div64(a.n * g, 128), dim3(128), 1, s, z, gz, a); };
-            // a warp holds rows of up to 128 windows: bf16 8192 x 1000 takes 18.2 us, with blocks from 32 windows on 20.6
+            // a warp holds rows of up to 256 windows, 8 a lane (bf16 30000 x 2000: 63 us, in blocks 67; 16000 x 4096, 512
+            // windows, by a warp 74, in blocks 66)
             if (w <= 4) return group(rows_group_kernel<T, 1, 4>, 4);
             if (w <= 16) return group(rows_group_kernel<T, 1, 16>, 16);
             if (w <= 32) return group(rows_group_kernel<T, 1, 32>, 32);
             if (w <= 64) return group(rows_group_kernel<T, 2, 32>, 32);
             if (w <= 128) return group(rows_group_kernel<T, 4, 32>, 32);
+            if (w <= 256) return group(rows_group_kernel<T, 8, 32>, 32);
             auto threads = [](int64_t k) { return dim3((unsigned)(ceil_div64(k, 32) * 32)); };
             // every window whole: rows on 16 bytes that fill the threads' windows
             const bool even = aligned && a.v % VEC == 0 &&
                               (gz == nullptr || (reinterpret_cast<uintptr_t>(gz) % 16 == 0 && (a.n == 1 || a.gn % VEC == 0)));
-            auto block = [&](auto full, auto shifted, int nv, int parts) {
-                const dim3 t = threads(ceil_div64(w, nv * parts));
-                return launch(even && (int64_t)t.x * nv * parts == w ? full : shifted, a.n * parts, t, parts, s, z, gz, a, parts);
+            auto block = [&](int parts) {
+                const dim3 t = threads(ceil_div64(w, kWindows * parts));
+                return launch(even && (int64_t)t.x * kWindows * parts == w ? rows_block_kernel<T, kFull>
+                                                                           : rows_block_kernel<T, kShifted>,
+                              a.n * parts, t, parts, s, z, gz, a, parts);
             };
-            if (w <= 4 * kBlockMost) return block(rows_block_kernel<T, 4, kFull>, rows_block_kernel<T, 4, kShifted>, 4, 1);
+            // 8 windows a thread (with 4, bf16 16000 x 4096 takes 80 us instead of 66, fp32 8000 x 4000 69 instead of 54);
+            // up to 512 threads without a cluster (bf16 4096 x 32768: 116 us; two blocks of 256 threads 121), then clusters of
+            // smaller blocks, which wait less for their slowest warp (bf16 2048 x 131072: 242 us; blocks of 512 threads 248)
+            if (w <= kWindows * 2 * kBlockMost) return block(1);
             for (int most = kBlockMost; most <= 2 * kBlockMost; most *= 2)
-                for (int parts = 1; parts <= 8; parts *= 2)
-                    if (w <= (int64_t)parts * 8 * most)
-                        return block(rows_block_kernel<T, 8, kFull>, rows_block_kernel<T, 8, kShifted>, 8, parts);
+                for (int parts = 2; parts <= 8; parts *= 2)
+                    if (w <= (int64_t)parts * kWindows * most)
+                        return block(parts);
         }
         return launch(rows_stream_kernel<T>, a.n, dim3(512), 1, s, z, gz, a);
     }
