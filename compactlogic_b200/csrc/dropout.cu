@@ -154,8 +154,8 @@ __global__ void __launch_bounds__(kThreads, kBlocks<T>) dropout_kernel(const T* 
 // blocks, by another shift in each row.  The threads put their blocks' keep masks, as wide as the elements, into shared
 // memory and each reads the mask of its own windows back from there, shifted, so that global memory sees whole windows.
 // Thread t of a block draws the entries from VEC (first - 1 + t) on, and owns window first + t of either row (the last
-// thread none); blockDim.x is at most a warp, so no warp waits for another.  gridDim.y * blockDim.y is a multiple of VEC / 2 wherever a thread has a second pair of rows: the shifts of
-// its rows are then the same all the way down.
+// thread none); blockDim.x is at most a warp, so no warp waits for another.  gridDim.y * blockDim.y is a multiple of VEC / 2
+// wherever a thread has a second pair of rows: the shifts of its rows are then the same all the way down.
 template <typename T, bool BATCH_INNER, bool RESCALE>
 __global__ void __launch_bounds__(kThreads, kBlocks<T>) dropout_shifted_kernel(const T* __restrict__ x, T* __restrict__ y,
                                                                             DropArgs a) {

@@ -298,8 +298,8 @@ template <int NP, int OPS, int STAGES> struct Ring {
     }
 };
 
-// Entries [c, c + N) of a parameter vector of d entries (on 16 bytes, or 32 for N = 8, unless `loose`); `past` outside it or without one.  Where
-// c is not a multiple of 4 they are cut out of aligned words.
+// Entries [c, c + N) of a parameter vector of d entries (on 16 bytes, or 32 for N = 8, unless `loose`); `past` outside it or
+// without one.  Where c is not a multiple of 4 they are cut out of aligned words.
 template <int N, Windows M>
 __device__ __forceinline__ void parameter(const float* __restrict__ v, int c, int d, bool loose, float past, float (&f)[N]) {
     if (v == nullptr) {
@@ -820,8 +820,8 @@ __device__ __forceinline__ void join(float& mean, float& m2, float m, float q, f
 
 // stats [2, chunks, n]: mean and sum of squared differences of each chunk's features.
 template <typename T, int V>
-__global__ void __launch_bounds__(kColThreads, 3) norm_strip_stats_kernel(const T* __restrict__ x, NormArgs<float> a, int64_t chunk,
-                                                                       float* __restrict__ stats) {
+__global__ void __launch_bounds__(kColThreads, 3)
+    norm_strip_stats_kernel(const T* __restrict__ x, NormArgs<float> a, int64_t chunk, float* __restrict__ stats) {
     constexpr int W = kColThreads / 32;
     __shared__ float sh[W][2][32 * V];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -928,10 +928,9 @@ __global__ void __launch_bounds__(1024) norm_strip_fold_kernel(const float* __re
 
 // y from x, mean and rstd; or gx from x, gy, and the folded sums c1, c2 (GRAD)
 template <typename T, int V, bool GRAD>
-__global__ void __launch_bounds__(kColThreads, GRAD ? 2 : 3) norm_strip_apply_kernel(const T* __restrict__ x, const T* __restrict__ gy,
-                                                                       T* __restrict__ y, NormArgs<float> a, int64_t chunk,
-                                                                          const float* mean, const float* rstd,
-                                                                          const float* c1, const float* c2) {
+__global__ void __launch_bounds__(kColThreads, GRAD ? 2 : 3)
+    norm_strip_apply_kernel(const T* __restrict__ x, const T* __restrict__ gy, T* __restrict__ y, NormArgs<float> a,
+                            int64_t chunk, const float* mean, const float* rstd, const float* c1, const float* c2) {
     constexpr int W = kColThreads / 32, B = 4;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t i = ((int64_t)blockIdx.x * 32 + lane) * V, j0 = blockIdx.y * chunk;
@@ -1076,7 +1075,8 @@ ColPlan col_plan(int64_t n, int64_t d, int elem, bool wide, bool backward) {
     p.v = wide ? 16 / elem : 1;
     p.strips = ceil_div64(n, 32 * p.v);
     // as many blocks as are resident at once (or more strips than that)
-    const int64_t resident = (int64_t)gpu_sms() * (backward ? 2 : 3), wanted = resident > p.strips ? resident / p.strips : 1, unit = kColThreads / 32 * kBatch;
+    const int64_t resident = (int64_t)gpu_sms() * (backward ? 2 : 3), unit = kColThreads / 32 * kBatch;
+    const int64_t wanted = resident > p.strips ? resident / p.strips : 1;
     p.chunk = ceil_div64(ceil_div64(d, wanted), unit) * unit;
     p.chunks = (int)ceil_div64(d, p.chunk);
     return p;
@@ -1329,7 +1329,8 @@ extern "C" int clb_layer_norm_forward(int dtype, const void* x, int64_t ldx, int
     switch (dtype) {
         case CLB_F32: return done(Norm<float>::forward(x, y, f, cols, workspace, s));
         case CLB_F64:
-            return done(Norm<double>::forward(x, y, args<double>(n, d, cols, ldx, ldy, 0, weight, bias, eps, mean, rstd), cols, workspace, s));
+            return done(Norm<double>::forward(x, y, args<double>(n, d, cols, ldx, ldy, 0, weight, bias, eps, mean, rstd), cols,
+                                              workspace, s));
         case CLB_BF16: return done(Norm<__nv_bfloat16>::forward(x, y, f, cols, workspace, s));
         default: return done(Norm<__half>::forward(x, y, f, cols, workspace, s));
     }

@@ -75,11 +75,11 @@ LAYOUTS = ["rows", "features", "padded", "padded_features", "strided"]
 
 
 # ------------------------------------------------------------------------------------------------------------- dropout
-def words(n, d, seed, offset):
-    """Philox4x32-10 as in its paper, in numpy: [n, d] words."""
+def words(n, d, seed, offset, first=0):
+    """Philox4x32-10 as in its paper, in numpy: [n, d] words, from the (even) row `first` on."""
     c = [np.zeros(((n + 1) // 2, (d + 1) // 2), dtype=np.uint64) for _ in range(4)]
     c[0] += np.arange((d + 1) // 2, dtype=np.uint64)[None, :]
-    c[1] += np.arange((n + 1) // 2, dtype=np.uint64)[:, None]
+    c[1] += np.arange(first // 2, first // 2 + (n + 1) // 2, dtype=np.uint64)[:, None]
     c[2] += np.uint64(offset & 0xFFFFFFFF)
     c[3] += np.uint64(offset >> 32)
     k0, k1 = seed & 0xFFFFFFFF, seed >> 32
@@ -734,6 +734,54 @@ def test_training_step_under_a_graph():
     torch.cuda.synchronize()
     for w, g in zip(want, got):
         assert (w - g).abs().max() <= 1e-5 * w.abs().max()
+
+
+@pytest.mark.parametrize("layout", ["rows", "features"])
+def test_offsets_past_32_bits(layout):
+    """Tensors of more than 2^31 elements: the last rows are right."""
+    n, d = (33000, 65536) if layout == "rows" else (65536, 33000)
+    free, _ = torch.cuda.mem_get_info()
+    if free < 40 << 30:
+        pytest.skip("needs 40 GB of device memory")
+    base = torch.empty(n, d, dtype=torch.bfloat16, device="cuda") if layout == "rows" else \
+        torch.empty(d, n, dtype=torch.bfloat16, device="cuda").t()
+    base.fill_(0.5)
+    tail = rand((6, d), 1, torch.bfloat16)
+    base[-6:] = tail
+    x = base.requires_grad_()
+    y = cl.dropout(x, 0.25, seed=3, rescale=False)
+    keep = torch.from_numpy(words(6, d, 3, 0, first=n - 6).astype(np.int64)).cuda() >= round(0.25 * 2 ** 32)
+    assert torch.equal(y[-6:], torch.where(keep, tail, torch.zeros((), dtype=tail.dtype, device="cuda")))
+    del y
+    gy = torch.zeros_like(base)
+    gy[-6:] = rand((6, d), 2, torch.bfloat16)
+    y = cl.layer_norm(x)
+    gx, = torch.autograd.grad(y, x, gy)
+    y64, h, mu, r, w64, t, gx64, *_ = norm64(tail, None, None, 1e-5, gy[-6:])
+    spread = 1 + (mu.abs() + tail.double().abs().mean(1, keepdim=True)) * r + h.abs()
+    near(y[-6:], y64, EPS * steps(d) * spread, torch.bfloat16, "y")
+    big = t.abs() + t.abs().mean(1, keepdim=True) + (1 + h.abs()) * ((t * h).abs().mean(1, keepdim=True) +
+                                                                  (t.abs() * spread).mean(1, keepdim=True))
+    near(gx[-6:], gx64, 2 * EPS * steps(d) * r * big, torch.bfloat16, "gx")
+    del y, gx, gy
+    act = torch.zeros(n, dtype=torch.int64, device="cuda")
+    act[-6:] = torch.tensor([0, 5, d - 1, d // 2, 7, d - 3], device="cuda")
+    up = torch.zeros(n, device="cuda")
+    up[-6:] = 1.5
+    lp = cl.action_log_probs(x, act)
+    gz, = torch.autograd.grad(lp, x, up)
+    full, want = logits64(tail, act[-6:], torch.ones(6, dtype=torch.bool, device="cuda"), 1.0)
+    slack = row_slack(tail, want, 1.0, torch.bfloat16)
+    near(lp[-6:], want, slack, torch.float32, "logp")
+    grad = -1.5 * full.exp()
+    grad[torch.arange(6, device="cuda"), act[-6:]] += 1.5
+    near(gz[-6:], grad, grad_slack(full, up[-6:].double(), slack, torch.bfloat16), torch.bfloat16, "gz")
+    assert (gz[:-6:997] == 0).all()
+    del gz
+    r = cl.policy_loss(x, act, up, lp.detach(), reduction="sum")
+    gz, = torch.autograd.grad(r.loss, x)
+    # ratios of exactly 1: the slope is -1.5
+    near(gz[-6:], -grad, grad_slack(full, up[-6:].double(), slack, torch.bfloat16), torch.bfloat16, "policy gz")
 
 
 def test_status_codes():
