@@ -198,9 +198,7 @@ class _LayerNormFn(torch.autograd.Function):
         x, inner, ld = _matrix(x)
         gy, g_inner, ldg = _matrix(gy)
         if g_inner != inner:
-            if n > 1 and d > 1:
-                gy = gy.t().contiguous().t() if inner else gy.contiguous()
-            ldg = (gy.stride(1) if d > 1 else n) if inner else (gy.stride(0) if n > 1 else d)
+            gy, ldg = (gy.t().contiguous().t(), n) if inner else (gy.contiguous(), d)
         acc = _ACC[x.dtype]
         need = ctx.needs_input_grad
         gx = _like(x, inner) if need[0] else None

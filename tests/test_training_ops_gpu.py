@@ -370,6 +370,31 @@ def test_layer_norm_repeats_its_bits(layout):
     assert torch.equal(a[4], b[4]) and all(torch.equal(p, q) for p, q in zip(a[5], b[5]))
 
 
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("n,d", [(1, 1), (1, 2), (1, 8), (1, 784), (1, 5001), (5, 1)])
+def test_layer_norm_of_one_row_or_one_feature(n, d, dtype, layout):
+    """Where an axis has one entry its stride says nothing: every storage of the input with every one of the gradient."""
+    for gy_layout in LAYOUTS:
+        check_norm(n, d, dtype, layout, gy_layout=gy_layout)
+
+
+def test_layer_norm_of_one_row_between_stack_and_cat():
+    """Gradients of one row as autograd hands them over: columns of a wider matrix."""
+    d = 96
+    x, w, b = rand((1, d), 1).requires_grad_(), rand((d,), 2, shift=1.0).requires_grad_(), rand((d,), 3).requires_grad_()
+    for join, g in [(lambda y: torch.stack([y, 2 * y.detach()], -1), rand((1, d, 2), 4)),
+                    (lambda y: torch.cat([y.t(), y.detach().t(), y.detach().t()], 1), rand((d, 3), 5))]:
+        y = cl.layer_norm(x, w, b)
+        got = torch.autograd.grad(join(y), (x, w, b), g)
+        gy = g[..., 0].reshape(1, d).clone()
+        want = torch.autograd.grad(cl.layer_norm(x, w, b), (x, w, b), gy)
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+        *_, gx, gw, gb = norm64(x, w, b, 1e-5, gy)
+        for p, q in zip(got, (gx, gw, gb)):
+            assert (p.double() - q).abs().max() <= EPS * 16 * steps(d) * (1 + q.abs().max())
+
+
 # -------------------------------------------------------------------------------------------------------------- losses
 def logits64(z, actions, live, temperature):
     z = z.detach().double() / temperature
