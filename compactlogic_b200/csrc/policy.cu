@@ -223,30 +223,28 @@ template <typename T, int NV, int STRIDE, Windows M> struct RowPart {
         const float m = fmaxf(top(), -INFINITY);  // NaN where all entries are
         r.m = m;
         const float safe = m == -INFINITY ? 0.f : m;
+        // The difference first: one multiply-add with a product -m * factor would leave that product's rounding in every
+        // exponent of the row, all the more the larger the logits or the smaller T (bf16 2048 x 131072: 242 us; so 240).
         float f[VEC], s[4] = {};
-        if (fabsf(safe) < 1e37f) {  // the product with the factor stays finite: one multiply-add an element
-            const float mk = safe * factor;
 #pragma unroll
-            for (int u = 0; u < NV; ++u) {
-                x[u].get(f);
+        for (int u = 0; u < NV; ++u) {
+            x[u].get(f);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) s[j & 3] += soft_exp(fmaf(f[j], factor, -mk));
-            }
-        } else {
-#pragma unroll
-            for (int u = 0; u < NV; ++u) {
-                x[u].get(f);
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) s[j & 3] += soft_exp((f[j] - safe) * factor);
-            }
+            for (int j = 0; j < VEC; ++j) s[j & 3] += soft_exp((f[j] - safe) * factor);
         }
         r.s = (s[0] + s[1]) + (s[2] + s[3]);
+    }
+    // Between sum and grad: without it the converted logits of 16 bits, twice the registers, are kept from one to the other and
+    // spill (bf16 2048 x 131072: 280 us).
+    __device__ __forceinline__ void pin() {
+#pragma unroll
+        for (int u = 0; u < NV; ++u)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) asm volatile("" : "+r"(x[u].w[k]));
     }
     // the row's gradient without the chosen action's own term; `same`: out's windows lie as the row's
     __device__ __forceinline__ void grad(T* __restrict__ out, int c, bool same, int v, const RowGrad<float>& g,
                                          float factor) const {
-        const bool tame = fabsf(g.m) < 1e37f;
-        const float mk = g.m * factor;
         const unsigned whole = same && v >= VEC ? v - VEC + 1 : 0;
         T* at = out + c;
 #pragma unroll
@@ -254,13 +252,8 @@ template <typename T, int NV, int STRIDE, Windows M> struct RowPart {
             if (M != kFull && c + u * STEP >= v) break;
             float f[VEC];
             x[u].get(f);
-            if (tame) {
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) f[j] = g.w * soft_exp(fmaf(f[j], factor, -mk));
-            } else {
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) f[j] = g.w * soft_exp((f[j] - g.m) * factor);
-            }
+            for (int j = 0; j < VEC; ++j) f[j] = g.w * soft_exp((f[j] - g.m) * factor);
             Pack<T, VEC> y;
             y.put(f);
             put(at + u * STEP, c + u * STEP, whole, v, y);
@@ -328,6 +321,7 @@ __global__ void __launch_bounds__(128) rows_group_kernel(const T* __restrict__ z
         return;
     }
     const RowGrad<float> g = row_grad(a, slope, r.m, r.s);
+    part.pin();
     part.grad(out, c, same, v, g, a.factor);
     const int64_t act = a.actions[i];
     if (act >= 0 && act < v && ((int)act + shift) / Part::VEC % G == lane) put_action(out, row, act, g, a.factor);
@@ -390,6 +384,7 @@ __global__ void __launch_bounds__(512, 2) rows_block_kernel(const T* __restrict_
     if (gz == nullptr) return;
     __syncthreads();
     const RowGrad<float> g = shared;
+    part.pin();
     part.grad(out, c, same, v, g, a.factor);
     const int64_t act = a.actions[i];
     if (act >= 0 && act < v) {
@@ -440,11 +435,9 @@ __global__ void __launch_bounds__(512) rows_stream_kernel(const T* __restrict__ 
         __syncthreads();
         const RowGrad<A> g = shared;
         const int64_t act = a.actions[i];
-        const bool tame = sizeof(A) == 4 && fabs(g.m) < (A)1e37;  // as RowPart::grad, bit for bit
-        const A mk = g.m * a.factor;
         for (j = threadIdx.x; j < a.v; j += blockDim.x) {
             const A f = to_acc(row[j]);
-            const A e = g.w * soft_exp(tame && j != act ? fma(f, a.factor, -mk) : (f - g.m) * a.factor);
+            const A e = g.w * soft_exp((f - g.m) * a.factor);
             out[j] = from_acc<T>(j == act ? g.c + e : e);
         }
     }

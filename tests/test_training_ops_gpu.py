@@ -625,6 +625,71 @@ def test_masked_logits(v, dtype, layout):
     assert (r.log_probs[4:7] == 0).all() and (r.ratio[4:7] == 0).all() and (r.kl[4:7] == 0).all()
 
 
+# A row's form by its length: lanes of a warp, a warp, a block, a cluster, and beyond a cluster (read twice).
+LENGTHS = [3, 17, 47, 300, 1777, 3000, 20000, 50001, 131072, 600001]
+
+
+def loss_inputs(z, seed=30, temperature=1.0):
+    """What ``policy_inputs`` makes, for given logits."""
+    n, v = z.shape
+    acc = torch.float64 if z.dtype == torch.float64 else torch.float32
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    act = torch.randint(0, v, (n,), generator=g, device="cuda")
+    act[0] = z[0].argmax()
+    lp = torch.log_softmax(z.double() / temperature, 1).gather(1, act[:, None])[:, 0]
+    step = torch.rand(n, generator=g, device="cuda", dtype=torch.float64) * 0.15
+    step = torch.where(torch.rand(n, generator=g, device="cuda") < 0.4, step + 0.27, step)
+    old = (lp + torch.where(torch.rand(n, generator=g, device="cuda") < 0.5, step, -step)).to(acc)
+    refs = (lp + rand((n,), seed + 2, torch.float64, 0.5)).to(acc)
+    return z, act, rand((n,), seed + 1, acc, 1.0, 0.3), old, refs, None
+
+
+@pytest.mark.parametrize("layout", ["rows", "padded", "features"])
+@pytest.mark.parametrize("v", LENGTHS)
+@pytest.mark.parametrize("shift,scale,temperature", [(1e3, 2.0, 1.0), (-1e5, 2.0, 1.0), (1e6, 2.0, 1.0), (0.0, 3.0, 0.01),
+                                                     (30.0, 0.05, 0.01)])
+def test_losses_of_logits_far_from_zero(v, shift, scale, temperature, layout):
+    """What the logits have in common cancels exactly, in the sum, in the gradient and in the action's own entry, whatever
+    the row's form, and a small temperature does not magnify its rounding."""
+    n = 5
+    z = laid(rand((n, v), 40, torch.float32, scale, shift), layout)
+    z, act, *_ = inputs = loss_inputs(z, temperature=temperature)
+    check_policy(n, v, torch.float32, layout, temperature=temperature, inputs=inputs)
+    z = z.detach().requires_grad_()
+    lp = cl.action_log_probs(z, act, temperature=temperature)
+    up = rand((n,), 21)
+    gz, = torch.autograd.grad(lp, z, up)
+    full, want = logits64(z, act, torch.ones(n, dtype=torch.bool, device="cuda"), temperature)
+    slack = row_slack(z, want, temperature, torch.float32)
+    near(lp, want, slack, torch.float32, "logp")
+    c = up.double() / temperature
+    grad = -c[:, None] * full.exp()
+    grad[torch.arange(n, device="cuda"), act] += c
+    near(gz, grad, grad_slack(full, c, slack, torch.float32), torch.float32, "gz")
+
+
+@pytest.mark.parametrize("layout", ["rows", "padded", "features"])
+@pytest.mark.parametrize("dtype", LOW)
+@pytest.mark.parametrize("v", LENGTHS)
+def test_rows_filled_with_one_value(v, dtype, layout):
+    """A mask by a large finite value that leaves nothing: every class has probability 1 / v, at any temperature."""
+    fills = [-1e4, 6e4] if dtype == torch.float16 else [-1e4, -1e9, 1e30, -1e37, -3e38]
+    z = laid(torch.tensor(fills, device="cuda", dtype=dtype)[:, None].expand(-1, v), layout).requires_grad_()
+    n = len(fills)
+    act = torch.arange(n, device="cuda") * 7 % v
+    for temperature in (1.0, 0.02):
+        lp = cl.action_log_probs(z, act, temperature=temperature)
+        assert (lp.double() + math.log(v)).abs().max() <= EPS * (steps(v) + 4 * math.log(v))
+        gz, = torch.autograd.grad(lp.sum(), z)
+        want = torch.full((n, v), -1.0 / v, dtype=torch.float64, device="cuda")
+        want[torch.arange(n, device="cuda"), act] += 1.0
+        near(gz, want / temperature, EPS * (steps(v) + 16) * (want.abs() + 1 / v) / temperature, dtype, "gz")
+        r = cl.policy_loss(z, act, torch.full((n,), -2.0, device="cuda"), lp.detach(), temperature=temperature)
+        gz, = torch.autograd.grad(r.loss, z)     # ratios of 1: the slope is the negative advantage
+        near(gz, want * 2 / n / temperature, EPS * (steps(v) + 16) * (want.abs() + 1 / v) * 2 / n / temperature, dtype,
+             "policy gz")
+
+
 @pytest.mark.parametrize("layout", ["rows", "features"])
 @pytest.mark.parametrize("v", [10, 3000])
 def test_policy_loss_edges(v, layout):
