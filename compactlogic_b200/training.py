@@ -8,8 +8,10 @@
 All four take the layers' own storage (``[batch, features]`` views of feature-major memory) and ordinary row-major tensors
 alike, without copies, and run on the current stream.  A strided tensor that is neither is copied first.
 """
+from collections import deque
 from functools import lru_cache
 from typing import NamedTuple, Optional, Tuple, Union
+from weakref import WeakValueDictionary
 
 import torch
 
@@ -123,12 +125,27 @@ def dropout(x: torch.Tensor, p: float = 0.5, *, seed: int, offset: int = 0, resc
     return _dropout(x, p, rescale, seed, offset, None)
 
 
+def _generator_place(index: int):
+    """Where torch's generator of a GPU stands, which moves on by one draw; None while a graph is captured."""
+    if torch.cuda.is_current_stream_capturing():
+        return None
+    generator = torch.cuda.default_generators[index]
+    at = generator.get_offset()
+    generator.set_offset(at + 4)
+    return index, generator.initial_seed(), at
+
+
 class LogicDropout(torch.nn.Module):
     """``dropout`` between logic layers, a new mask for each training pass; the identity in eval mode.
 
     The buffer ``rng_state`` (int64 {seed, offset}) advances on the device, so a captured training step
     (``compactlogic_b200.graph``) draws a new mask at each replay, and a loaded checkpoint continues the sequence.  ``seed``
-    defaults to a draw from torch's generator.  Passes of one module on several streams at once are not ordered."""
+    defaults to a draw from torch's generator.  Passes of one module on several streams at once are not ordered.
+
+    A pass that activation checkpointing (``torch.utils.checkpoint``, either form) computes again draws the mask of the pass
+    that it repeats.  The two are matched by where torch's CUDA generator stands, which checkpointing puts back
+    (``preserve_rng_state``); passes that may be repeated, those without gradients or under saved-tensor hooks, move it on as
+    torch's dropout does.  A forward pass inside a backward pass that matches none, or two, raises."""
 
     def __init__(self, p: float = 0.5, rescale: bool = True, seed: Optional[int] = None):
         super().__init__()
@@ -140,15 +157,50 @@ class LogicDropout(torch.nn.Module):
             raise ValueError("LogicDropout: seed must be in [0, 2^63)")
         self.p, self.rescale = float(p), bool(rescale)
         self.register_buffer("rng_state", torch.tensor([seed, 0], dtype=torch.int64))
+        self._forget()
+
+    def _forget(self):
+        # {generator place: {seed, offset}} of passes that may be repeated.  The pass's autograd node keeps the entry; of those
+        # without a node the newest are kept.
+        self._passes = WeakValueDictionary()
+        self._loose = deque(maxlen=1024)
+
+    def __getstate__(self):
+        return {k: v for k, v in self.__dict__.items() if k not in ("_passes", "_loose")}
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._forget()
+
+    def _draw(self, x):
+        """The generator state {seed, offset} of one pass, on the device."""
+        again = torch._C._current_graph_task_id() != -1  # a forward pass inside a backward pass
+        node = x.requires_grad and torch.is_grad_enabled()
+        place = None
+        if again or not node or torch._C._autograd._top_saved_tensors_default_hooks(True) is not None:
+            place = _generator_place(x.get_device())
+        if again:
+            used = self._passes.get(place)
+            if used is None or used.shared_place:
+                raise RuntimeError("LogicDropout: a pass inside a backward pass has to recompute one earlier pass, which torch's "
+                                   "CUDA generator tells; checkpoint with preserve_rng_state=True, and do not seed the "
+                                   "generator alike for two passes in flight")
+            return used
+        used = torch.empty(2, dtype=torch.int64, device=x.device)
+        L.call("clb_dropout_advance", self.rng_state.data_ptr(), used.data_ptr(), _stream(x.get_device()))
+        if place is not None:
+            used.shared_place = place in self._passes
+            self._passes[place] = used
+            if not node:
+                self._loose.append(used)
+        return used
 
     def forward(self, x):
         if not self.training or self.p == 0.0:
             return x
         _check("LogicDropout", x)
         _same_device("LogicDropout", x, "rng_state", self.rng_state)
-        used = torch.empty(2, dtype=torch.int64, device=x.device)
-        L.call("clb_dropout_advance", self.rng_state.data_ptr(), used.data_ptr(), _stream(x.get_device()))
-        return _dropout(x, self.p, self.rescale, 0, 0, used)
+        return _dropout(x, self.p, self.rescale, 0, 0, self._draw(x))
 
     def extra_repr(self):
         return f"p={self.p}, rescale={self.rescale}"

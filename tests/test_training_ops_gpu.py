@@ -188,6 +188,83 @@ def test_dropout_module_under_a_graph():
         assert torch.equal(t, dropped(x, 0.5, 5, 1 + k, True))
 
 
+def checkpointed(reentrant):
+    from torch.utils.checkpoint import checkpoint
+    return (lambda f, *a: f(*a)) if reentrant is None else (lambda f, *a: checkpoint(f, *a, use_reentrant=reentrant))
+
+
+@pytest.mark.parametrize("shape", [(48, 64), (6, 4, 5, 7)])
+@pytest.mark.parametrize("reentrant", [True, False])
+def test_dropout_module_recomputed_by_activation_checkpointing(reentrant, shape):
+    """A recomputed pass draws the mask of the pass that it repeats: several passes of one module in a block, several
+    blocks in flight, an input that needs no gradient, and passes outside."""
+    def run(how):
+        torch.manual_seed(0)
+        torch.cuda.manual_seed(1)
+        wrap = checkpointed(how)
+        m = cl.LogicDropout(0.4, seed=9).cuda()
+        w = rand(shape[1:], 1).requires_grad_()
+        xs = [rand(shape, 2 + k).requires_grad_(k > 0) for k in range(3)]
+        with torch.no_grad():
+            m(xs[0])                                                   # a rollout
+        ys = [wrap(lambda x, w: m(torch.tanh(m(x) * w) * 2), x, w) for x in xs]
+        last = m(ys[0] * ys[1])
+        noise = torch.rand(4, device="cuda")                           # torch's own sequence
+        ((last ** 2).sum() + sum((y ** 2).sum() for y in ys)).backward()
+        after = m(xs[0].detach())
+        return ys + [last, after] + [x.grad for x in xs[1:]] + [m.rng_state], w.grad, noise
+
+    want, gw, _ = run(None)
+    got, gw2, noise = run(reentrant)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    assert want[-1].tolist() == [9, 9]
+    assert (gw - gw2).abs().max() <= 1e-6 * gw.abs().max()             # summed over the blocks in another order
+
+
+@pytest.mark.parametrize("reentrant", [True, False])
+def test_dropout_module_refuses_a_recomputation_that_it_cannot_repeat(reentrant):
+    """Without torch's generator put back, or where it stood at the same place in two passes, a recomputed pass cannot
+    tell which one it repeats."""
+    from torch.utils.checkpoint import checkpoint
+    m = cl.LogicDropout(0.5, seed=3).cuda()
+    x = rand((8, 8), 1).requires_grad_()
+    y = checkpoint(m, x, use_reentrant=reentrant, preserve_rng_state=False)
+    torch.rand(8, 8, device="cuda")
+    if reentrant:
+        with pytest.raises(RuntimeError, match="recomput"):
+            (y * y).sum().backward()
+    else:  # dropout alone saves nothing that would have to be computed again
+        gx, = torch.autograd.grad((y * y).sum(), x)
+        assert torch.equal(gx, 4 * dropped(x.detach(), 0.5, 3, 0, True))
+    y = checkpoint(lambda t: m(t) * t, x, use_reentrant=reentrant, preserve_rng_state=False)
+    torch.rand(8, 8, device="cuda")
+    with pytest.raises(RuntimeError, match="recomput"):
+        (y * y).sum().backward()
+    torch.cuda.manual_seed(5)
+    a = checkpoint(lambda t: m(t) * t, x, use_reentrant=reentrant)
+    torch.cuda.manual_seed(5)
+    b = checkpoint(lambda t: m(t) * t, x, use_reentrant=reentrant)
+    with pytest.raises(RuntimeError, match="recomput"):
+        (a + b).sum().backward()
+
+
+def test_dropout_module_copies_and_pickles():
+    import copy
+    import io
+    import pickle
+    m = cl.LogicDropout(0.5, seed=3).cuda()
+    x = torch.ones(8, 64, device="cuda", requires_grad=True)
+    with torch.no_grad():
+        m(x)
+    y = m(x)
+    file = io.BytesIO()
+    torch.save(m, file)
+    file.seek(0)
+    for other in (copy.deepcopy(m), pickle.loads(pickle.dumps(m)), torch.load(file, weights_only=False)):
+        assert torch.equal(other(x), dropped(torch.ones_like(x), 0.5, 3, 2, True))
+    assert torch.equal(y, dropped(torch.ones_like(x), 0.5, 3, 1, True))
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_dropout_between_logic_layers(dtype):
     """The layers' gradients through dropout equal those of the same network with the mask multiplied in by torch; with
