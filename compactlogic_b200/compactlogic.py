@@ -78,6 +78,12 @@ class LogicLayer(torch.nn.Module):
         assert xt.shape[0] == self.in_dim, (xt.shape, self.in_dim)
         return xt
 
+    @staticmethod
+    def _out_slot(xt):
+        # none without a graph: nothing would read it (the first pass of reentrant activation checkpointing, whose consumers
+        # would then hand their gradient to a layer that has no backward pass)
+        return GradSlot() if xt.dtype in (torch.bfloat16, torch.float16) and torch.is_grad_enabled() else None
+
     def _weights_for(self, dtype):
         return self.weights.double() if dtype == torch.float64 else self.weights
 
@@ -91,7 +97,7 @@ class LogicLayer(torch.nn.Module):
             k, tau = self._fused_groupsum
             acc = LogicGroupSumFn.apply(xt, w, spec, k, _group_size(self.out_dim, k), in_slot)
             return acc.transpose(0, 1) / tau
-        out_slot = GradSlot() if xt.dtype in (torch.bfloat16, torch.float16) else None
+        out_slot = self._out_slot(xt)
         y = LogicLayerFn.apply(xt, w, spec, in_slot, out_slot).transpose(0, 1)
         if out_slot is not None:
             y._clb_slot = out_slot
@@ -591,7 +597,7 @@ class ConvLayer(LogicLayer):
         in_slot = getattr(x, "_clb_slot", None)
         xt = self._to_feature_major(x)
         spec = self._layer_spec(xt.device)
-        out_slot = GradSlot() if xt.dtype in (torch.bfloat16, torch.float16) else None
+        out_slot = self._out_slot(xt)
         y = self._to_public(LogicLayerFn.apply(xt, self._weights_for(xt.dtype), spec, in_slot, out_slot))
         if out_slot is not None:
             y._clb_slot = out_slot

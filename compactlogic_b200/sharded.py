@@ -274,7 +274,8 @@ class WidthShardedLogicLayer(LogicLayer):
         xt = self._to_feature_major(x)
         out_slot = PeerGradSlot()
         y = _WidthShardedFn.apply(xt, self._weights_for(xt.dtype), self, in_slot, out_slot).transpose(0, 1)
-        y._clb_peer_slot = out_slot
+        if torch.is_grad_enabled():  # as LogicLayer._out_slot
+            y._clb_peer_slot = out_slot
         return y
 
     def _forward_eval(self, x):

@@ -297,6 +297,29 @@ def test_dropout_between_logic_layers(dtype):
         assert (g - w).abs().max() <= tol * w.abs().max()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("reentrant", [True, False])
+def test_logic_layers_and_dropout_recomputed(reentrant, dtype):
+    """Layers and dropout in checkpointed blocks: the gradients of the plain network."""
+    def run(how):
+        torch.manual_seed(0)
+        wrap = checkpointed(how)
+        a, b, c = cl.LogicLayer(64, 96).cuda(), cl.LogicLayer(96, 80).cuda(), cl.LogicLayer(80, 60).cuda()
+        m = cl.LogicDropout(0.25, rescale=False, seed=4).cuda()
+        x = rand((40, 64), 1).sigmoid().to(dtype).requires_grad_()
+        y = cl.GroupSum(6, tau=2.0)(c(wrap(lambda t: b(m(a(t))), x)))
+        (y * rand(y.shape, 2, dtype)).sum().backward()
+        return y, [x.grad] + [t.weights.grad for t in (a, b, c)]
+
+    want, grads = run(None)
+    got, again = run(reentrant)
+    assert torch.equal(want, got)
+    # the gradient that a recomputed block is given is autograd's, rounded to the activations' type: 40 samples' terms, U each
+    tol = 40 * U[dtype] if reentrant and dtype != torch.float32 else 1e-5
+    for g, w in zip(again, grads):
+        assert (g.double() - w.double()).abs().max() <= tol * w.double().abs().max()
+
+
 # ---------------------------------------------------------------------------------------------------------- layer norm
 def norm64(x, w, b, eps, gy=None):
     x = x.detach().double()
