@@ -304,6 +304,25 @@ def _backward_gather(xt, weights, spec, mode, gy, gs_grad, gs_size, gs_scale, ne
     return gx, gw
 
 
+class _FirstOrder(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, grad, what, *sources):
+        ctx.what = what
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, *unused):
+        raise RuntimeError(f"{ctx.what}: the second derivative is not implemented")
+
+
+def first_order(what: str, grad, *sources):
+    """A gradient that kernels made from ``sources``.  Under create_graph it raises when it is differentiated with respect to
+    one of them, where it would otherwise count as a constant."""
+    if grad is None or not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in sources):
+        return grad
+    return _FirstOrder.apply(grad.detach(), what, *sources)
+
+
 class GradSlot:
     """fp32 gradient hand-over between two logic layers whose activations are low precision (bf16 / fp16).
 

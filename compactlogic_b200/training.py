@@ -7,6 +7,8 @@
 
 All four take the layers' own storage (``[batch, features]`` views of feature-major memory) and ordinary row-major tensors
 alike, without copies, and run on the current stream.  A strided tensor that is neither is copied first.
+
+First derivatives are complete.  Of second ones (create_graph) only dropout's exist; the others raise when they are asked for.
 """
 from collections import deque
 from functools import lru_cache
@@ -16,7 +18,7 @@ from weakref import WeakValueDictionary
 import torch
 
 from . import _lib as L
-from .functional import GradSlot, _incoming_grad
+from .functional import GradSlot, _incoming_grad, first_order
 
 __all__ = ["LogicDropout", "LogicLayerNorm", "PolicyLoss", "action_log_probs", "dropout", "layer_norm", "policy_loss"]
 
@@ -41,6 +43,11 @@ def _matrix(x: torch.Tensor) -> Tuple[torch.Tensor, int, int]:
     if (sn == 1 or n <= 1) and (sd >= n or d <= 1):
         return x, 1, sd if d > 1 else n
     return x.contiguous(), 0, d
+
+
+def _dense(x: torch.Tensor) -> torch.Tensor:
+    """``x``, or the copy that ``_matrix`` makes of it, within the graph."""
+    return x if x.is_contiguous() else _matrix(x)[0]
 
 
 def _like(x: torch.Tensor, inner: int) -> torch.Tensor:
@@ -87,7 +94,10 @@ class _DropoutFn(torch.autograd.Function):
         slot = ctx.out_slot
         if slot is not None and slot.grad is not None:
             gy = _incoming_grad(gy.t(), slot, torch.float32).t()
-        gx = _drop(gy, *ctx.args)
+        if gy.requires_grad and torch.is_grad_enabled():  # create_graph: linear in gy
+            gx = _DropoutFn.apply(gy, *ctx.args, None, None)
+        else:
+            gx = _drop(gy, *ctx.args)
         if ctx.in_slot is not None:
             ctx.in_slot.add(gx.float().t())
             gx = torch.zeros((), dtype=ctx.dtype, device=gx.device).expand(ctx.shape)
@@ -245,7 +255,7 @@ class _LayerNormFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, gy):
         x, weight = ctx.saved_tensors
-        stats = ctx.stats
+        stats, given = ctx.stats, gy
         n, d = x.shape
         x, inner, ld = _matrix(x)
         gy, g_inner, ldg = _matrix(gy)
@@ -264,7 +274,8 @@ class _LayerNormFn(torch.autograd.Function):
             n if inner else d, L.ptr(gw), L.ptr(gb), L.ptr(ws), nbytes, _stream(x.get_device()))
         if status:
             L.check(status, "clb_layer_norm_backward")
-        return gx, gw, gb, None
+        return (first_order("layer_norm", gx, x, weight, given), first_order("layer_norm", gw, x, given),
+                first_order("layer_norm", gb, given), None)
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
@@ -290,7 +301,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     bias = bias if bias is None or bias.is_contiguous() else bias.contiguous()
     flat = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     if grad and torch.is_grad_enabled():
-        y = _LayerNormFn.apply(flat, weight, bias, eps)
+        y = _LayerNormFn.apply(_dense(flat), weight, bias, eps)
     else:
         y = _norm_forward(flat, weight, bias, eps, False)[0]
     return y if x.dim() == 2 else y.reshape(x.shape)
@@ -391,7 +402,8 @@ class _LogProbFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, g):
         z, actions, mask = ctx.saved_tensors
-        return (_logit_grad(z, actions, mask, ctx.temperature, ctx.stats.data_ptr(), 0, 0, g, g.stride(0)), None, None, None)
+        gz = _logit_grad(z, actions, mask, ctx.temperature, ctx.stats.data_ptr(), 0, 0, g, g.stride(0))
+        return first_order("action_log_probs", gz, z, g), None, None, None
 
 
 def _check_temperature(what, temperature):
@@ -410,7 +422,7 @@ def action_log_probs(logits: torch.Tensor, actions: torch.Tensor, *, mask: Optio
     z, act, m, lead = _rows_of("action_log_probs", logits, actions, mask)
     _check_temperature("action_log_probs", temperature)
     if z.requires_grad and torch.is_grad_enabled():
-        logp = _LogProbFn.apply(z, act, m, temperature)
+        logp = _LogProbFn.apply(_dense(z), act, m, temperature)
     else:
         logp = _logp_forward(z, act, m, temperature, False)[0]
     return logp if len(lead) == 1 else logp.reshape(lead)
@@ -474,7 +486,7 @@ class _PolicyLossFn(torch.autograd.Function):
         gz, ctx.gz = ctx.gz, None
         gz = _logit_grad(z, actions, mask, ctx.temperature, at + n * size, at, at + 3 * n * size, g,
                          g.stride(0) if ctx.per_row else 0, gz)
-        return (gz,) + (None,) * 10
+        return (first_order("policy_loss", gz, z, g),) + (None,) * 10
 
 
 def policy_loss(logits: torch.Tensor, actions: torch.Tensor, advantages: torch.Tensor, old_log_probs: torch.Tensor, *,
@@ -508,12 +520,12 @@ def policy_loss(logits: torch.Tensor, actions: torch.Tensor, advantages: torch.T
                                   t.is_contiguous() and t.get_device() == dev):
             t = _per_row("policy_loss", name, t if t.dtype is acc else t.to(acc), z, lead)
         given.append(t)
-    args = (z, act, m, *given, low, high, kl_coef, temperature, reduction)
+    args = (act, m, *given, low, high, kl_coef, temperature, reduction)
     if z.requires_grad and torch.is_grad_enabled():
-        out = _PolicyLossFn.apply(*args)
+        out = _PolicyLossFn.apply(_dense(z), *args)
     else:
         with torch.no_grad():
-            out = _policy(*args, False)[:4]
+            out = _policy(z, *args, False)[:4]
     if len(lead) != 1:
         out = tuple(t if t is None or (i == 0 and reduction != "none") else t.reshape(lead) for i, t in enumerate(out))
     return PolicyLoss(*out)

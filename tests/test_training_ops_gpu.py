@@ -882,6 +882,43 @@ def test_loss_refusals():
         cl.policy_loss(z, act, adv, old, reduction="average")
 
 
+# --------------------------------------------------------------------------------------------------- second derivatives
+@pytest.mark.parametrize("layout", ["rows", "features"])
+def test_dropout_second_derivatives(layout):
+    x = laid(rand((9, 14), 1, torch.float64), layout).requires_grad_()
+    assert torch.autograd.gradgradcheck(lambda t: cl.dropout(t ** 3, 0.3, seed=2), (x,), eps=1e-6, atol=1e-7, rtol=1e-6)
+    assert torch.autograd.gradgradcheck(lambda t: cl.dropout((t ** 3).reshape(9, 2, 7), 0.3, seed=2), (x,), eps=1e-6,
+                                        atol=1e-7, rtol=1e-6)
+    g, = torch.autograd.grad(cl.dropout(x, 0.3, seed=2).sum(), x, create_graph=True)
+    again, = torch.autograd.grad((g * x).sum(), x)  # a gradient that is constant
+    assert torch.equal(again, g)
+
+
+@pytest.mark.parametrize("layout", ["rows", "features", "strided"])
+@pytest.mark.parametrize("name", ["layer_norm", "action_log_probs", "policy_loss", "policy_loss none"])
+def test_second_derivatives_are_refused(name, layout):
+    """A first derivative under create_graph is right; differentiated again it raises instead of leaving its term out."""
+    z, act, adv, old, refs, mask = policy_inputs(6, 20, torch.float32, layout)
+    w, b = rand((20,), 1).requires_grad_(), rand((20,), 2).requires_grad_()
+    z = z.requires_grad_()
+    calls = {"layer_norm": (lambda: cl.layer_norm(z, w, b), (z, w)),
+             "action_log_probs": (lambda: cl.action_log_probs(z, act), (z,)),
+             "policy_loss": (lambda: cl.policy_loss(z, act, adv, old, ref_log_probs=refs, kl_coef=0.1).loss, (z,)),
+             "policy_loss none": (lambda: cl.policy_loss(z, act, adv, old, reduction="none").loss, (z,))}
+    call, inputs = calls[name]
+    plain = torch.autograd.grad(call().sum(), inputs)
+    for up in (torch.ones_like(call()), torch.ones_like(call()).requires_grad_()):
+        for k, at in enumerate(inputs):
+            grads = torch.autograd.grad(call(), inputs, up, create_graph=True)
+            assert all(torch.equal(p, q) for p, q in zip(plain, grads))
+            with pytest.raises(RuntimeError, match="second derivative"):
+                torch.autograd.grad((grads[k] ** 2).sum() + (z ** 2).sum(), z)
+    # the bias's gradient is a sum of the incoming one: constant where that is
+    if name == "layer_norm":
+        gb, = torch.autograd.grad(call().sum(), b, create_graph=True)
+        assert torch.equal(torch.autograd.grad((gb * b).sum(), b)[0], gb)
+
+
 def test_operators_on_a_side_stream():
     """Work is enqueued on the current stream: results there equal those on the default one."""
     z, act, adv, old, refs, mask = policy_inputs(500, 1000, torch.bfloat16, "rows", masked=0.2)
