@@ -30,6 +30,19 @@ _BYTES = {torch.float32: 4, torch.float64: 8}
 # The small calls of a training step are bound by the host, so the paths below keep to one allocation where several buffers
 # live and die together, and look up the current stream by its device index.
 _stream = torch._C._cuda_getCurrentRawStream
+_device = torch._C._cuda_getDevice
+
+
+def _run(name: str, x: torch.Tensor, *args) -> None:
+    """One entry point, on the GPU of ``x`` (also where another is the current one) and the current stream there."""
+    index = x.get_device()
+    if index == _device():
+        status = getattr(L.lib(), name)(*args, _stream(index))
+    else:
+        with torch.cuda.device(index):
+            status = getattr(L.lib(), name)(*args, _stream(index))
+    if status:
+        L.check(status, name)
 
 
 # ------------------------------------------------------------------------------------------------------------ layouts
@@ -75,10 +88,8 @@ def _drop(x: torch.Tensor, p: float, rescale: bool, seed: int, offset: int, rng:
     n, d = x.shape
     if inner:
         n, d = d, n
-    status = L.lib().clb_dropout(L.dtype_code(x.dtype), x.data_ptr(), ld, n, d, inner, p, rescale, seed, offset,
-                                 rng.data_ptr() if rng is not None else 0, y.data_ptr(), d, _stream(x.get_device()))
-    if status:
-        L.check(status, "clb_dropout")
+    _run("clb_dropout", x, L.dtype_code(x.dtype), x.data_ptr(), ld, n, d, inner, p, rescale, seed, offset,
+         rng.data_ptr() if rng is not None else 0, y.data_ptr(), d)
     return y
 
 
@@ -197,7 +208,7 @@ class LogicDropout(torch.nn.Module):
                                    "generator alike for two passes in flight")
             return used
         used = torch.empty(2, dtype=torch.int64, device=x.device)
-        L.call("clb_dropout_advance", self.rng_state.data_ptr(), used.data_ptr(), _stream(x.get_device()))
+        _run("clb_dropout_advance", x, self.rng_state.data_ptr(), used.data_ptr())
         if place is not None:
             used.shared_place = place in self._passes
             self._passes[place] = used
@@ -237,11 +248,8 @@ def _norm_forward(x, weight, bias, eps, keep):
     stats = torch.empty(2 * n, dtype=acc, device=x.device) if keep else None
     at = stats.data_ptr() if keep else 0
     nbytes, ws = _norm_workspace(code, n, d, inner, 0, x.device)
-    status = L.lib().clb_layer_norm_forward(
-        code, x.data_ptr(), ld, n, d, inner, L.ptr(weight), L.ptr(bias), eps, y.data_ptr(), n if inner else d, at,
-        at + n * _BYTES[acc] if keep else 0, L.ptr(ws), nbytes, _stream(x.get_device()))
-    if status:
-        L.check(status, "clb_layer_norm_forward")
+    _run("clb_layer_norm_forward", x, code, x.data_ptr(), ld, n, d, inner, L.ptr(weight), L.ptr(bias), eps, y.data_ptr(),
+         n if inner else d, at, at + n * _BYTES[acc] if keep else 0, L.ptr(ws), nbytes)
     return y, x, stats
 
 
@@ -269,11 +277,8 @@ class _LayerNormFn(torch.autograd.Function):
         code = L.dtype_code(x.dtype)
         nbytes, ws = _norm_workspace(code, n, d, inner, 1, x.device)
         at = stats.data_ptr()
-        status = L.lib().clb_layer_norm_backward(
-            code, x.data_ptr(), ld, gy.data_ptr(), ldg, n, d, inner, L.ptr(weight), at, at + n * _BYTES[acc], L.ptr(gx),
-            n if inner else d, L.ptr(gw), L.ptr(gb), L.ptr(ws), nbytes, _stream(x.get_device()))
-        if status:
-            L.check(status, "clb_layer_norm_backward")
+        _run("clb_layer_norm_backward", x, code, x.data_ptr(), ld, gy.data_ptr(), ldg, n, d, inner, L.ptr(weight), at,
+             at + n * _BYTES[acc], L.ptr(gx), n if inner else d, L.ptr(gw), L.ptr(gb), L.ptr(ws), nbytes)
         return (first_order("layer_norm", gx, x, weight, given), first_order("layer_norm", gw, x, given),
                 first_order("layer_norm", gb, given), None)
 
@@ -370,11 +375,8 @@ def _logit_grad(z, actions, mask, temperature, stats, slope, scale, upstream, up
     fresh = gz is None
     if fresh:
         gz = _like(z, inner)
-    status = L.lib().clb_logit_grad(
-        L.dtype_code(z.dtype), z.data_ptr(), ld, n, v, inner, actions.data_ptr(), L.ptr(mask), temperature, stats, slope, scale,
-        upstream.data_ptr(), up_stride, not fresh, gz.data_ptr(), n if inner else v, _stream(z.get_device()))
-    if status:
-        L.check(status, "clb_logit_grad")
+    _run("clb_logit_grad", z, L.dtype_code(z.dtype), z.data_ptr(), ld, n, v, inner, actions.data_ptr(), L.ptr(mask),
+         temperature, stats, slope, scale, upstream.data_ptr(), up_stride, not fresh, gz.data_ptr(), n if inner else v)
     return gz
 
 
@@ -384,10 +386,8 @@ def _logp_forward(z, actions, mask, temperature, keep):
     acc = _ACC[z.dtype]
     logp = torch.empty(n, dtype=acc, device=z.device)
     stats = torch.empty(2 * n, dtype=acc, device=z.device) if keep else None
-    status = L.lib().clb_action_logp(L.dtype_code(z.dtype), z.data_ptr(), ld, n, v, inner, actions.data_ptr(), L.ptr(mask),
-                                     temperature, logp.data_ptr(), L.ptr(stats), _stream(z.get_device()))
-    if status:
-        L.check(status, "clb_action_logp")
+    _run("clb_action_logp", z, L.dtype_code(z.dtype), z.data_ptr(), ld, n, v, inner, actions.data_ptr(), L.ptr(mask),
+         temperature, logp.data_ptr(), L.ptr(stats))
     return logp, z, stats
 
 
@@ -452,13 +452,11 @@ def _policy(z, actions, mask, adv, old, ref, low, high, kl_coef, temperature, re
     at, size = kept.data_ptr(), _BYTES[acc]
     # the mean's and the sum's gradient is made in the same pass, for an upstream gradient of 1
     gz = _like(z, inner) if grad and not per_row else None
-    status = L.lib().clb_policy_loss(
-        L.dtype_code(z.dtype), z.data_ptr(), ld, n, v, inner, actions.data_ptr(), L.ptr(mask), adv.data_ptr(), old.data_ptr(),
-        L.ptr(ref), low, high, kl_coef, temperature, reduction == "mean", 0 if per_row else loss.data_ptr(),
-        at + 3 * n * size, loss.data_ptr() if per_row else at + (3 * n + 1) * size, logp.data_ptr(), ratio.data_ptr(),
-        L.ptr(kl), at if grad else 0, at + n * size if grad else 0, L.ptr(gz), n if inner else v, _stream(z.get_device()))
-    if status:
-        L.check(status, "clb_policy_loss")
+    _run("clb_policy_loss", z, L.dtype_code(z.dtype), z.data_ptr(), ld, n, v, inner, actions.data_ptr(), L.ptr(mask),
+         adv.data_ptr(), old.data_ptr(), L.ptr(ref), low, high, kl_coef, temperature, reduction == "mean",
+         0 if per_row else loss.data_ptr(), at + 3 * n * size, loss.data_ptr() if per_row else at + (3 * n + 1) * size,
+         logp.data_ptr(), ratio.data_ptr(), L.ptr(kl), at if grad else 0, at + n * size if grad else 0, L.ptr(gz),
+         n if inner else v)
     return loss, logp, ratio, kl, z, gz, kept
 
 

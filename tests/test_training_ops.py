@@ -78,3 +78,42 @@ def test_c_entry_points_refuse_without_a_gpu():
         a = list(grad)
         a[at] = value
         assert lib.clb_logit_grad(*a) == status, (at, value)
+
+
+def test_entry_points_run_on_their_inputs_gpu(monkeypatch):
+    """Where another GPU is the current one, the input's is made current around the call, and its stream is taken."""
+    from compactlogic_b200 import training as T
+    calls, entered = [], []
+
+    class On:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            entered.append(self.index)
+
+        def __exit__(self, *error):
+            entered.append(None)
+
+    class Lib:
+        def clb_probe(self, *args):
+            calls.append((args, list(entered)))
+            return self.status
+
+    class Input:
+        def get_device(self):
+            return 1
+
+    fake = Lib()
+    fake.status = L.CLB_OK
+    monkeypatch.setattr(T, "_stream", lambda index: 100 + index)
+    monkeypatch.setattr(T.torch.cuda, "device", On)
+    monkeypatch.setattr(T.L, "lib", lambda: fake)
+    for current in (0, 1):
+        monkeypatch.setattr(T, "_device", lambda: current)
+        T._run("clb_probe", Input(), 7, 8)
+    assert calls == [((7, 8, 101), [1]), ((7, 8, 101), [1, None])] and entered == [1, None]
+    fake.status = L.CLB_ERR_INVALID
+    fake.clb_last_error = lambda: b"no"
+    with pytest.raises(RuntimeError, match="clb_probe"):
+        T._run("clb_probe", Input())
