@@ -162,7 +162,13 @@ def ptr(t) -> int:
 
 
 def stream(device=None) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    """The current stream of a GPU, which has to be the current one: a launch goes to the current GPU, whatever the stream of
+    another one's default is."""
+    s = torch.cuda.current_stream(device)
+    if s.device_index != torch._C._cuda_getDevice():
+        raise RuntimeError(f"compactlogic_b200: the tensors are on cuda:{s.device_index}, but cuda:{torch._C._cuda_getDevice()} is "
+                           "the current device; make theirs current (torch.cuda.device or set_device)")
+    return s.cuda_stream
 
 
 def require_cuda(*tensors) -> None:

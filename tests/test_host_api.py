@@ -164,3 +164,20 @@ def test_fuse_groupsum_keeps_state_dict():
     cl.fuse_groupsum(model)
     assert list(model.state_dict()) == keys
     assert model[1]._fused_groupsum == (3, 1.0) and model[2].absorbed
+
+
+def test_streams_of_another_gpu_are_refused(monkeypatch):
+    """A launch goes to the current GPU: tensors of another one are refused before it."""
+    from compactlogic_b200 import _lib as L
+
+    class Stream:
+        cuda_stream = 77
+
+        def __init__(self, index):
+            self.device_index = index
+
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: Stream(0 if device is None else device))
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    assert L.stream() == 77 and L.stream(0) == 77
+    with pytest.raises(RuntimeError, match="cuda:1"):
+        L.stream(1)
