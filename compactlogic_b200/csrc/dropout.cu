@@ -342,11 +342,12 @@ extern "C" int clb_dropout(int dtype, const void* x, int64_t ldx, int64_t rows, 
     a.offset = offset;
     a.rng = rng;
     const double t = nearbyint(p * 4294967296.0);
-    a.threshold = t >= 4294967296.0 ? 0xFFFFFFFFu : (uint32_t)t;
+    const bool none = t >= 4294967296.0;  // no word is as large as 2^32: nothing is kept
+    a.threshold = none ? 0 : (uint32_t)t;
     a.scale = rescale && p < 1.0 ? 1.0 / (1.0 - p) : 1.0;
     cudaStream_t s = (cudaStream_t)stream;
     cudaError_t e = cudaSuccess;
-    if (p == 1.0) {  // no word is as large as 2^32: nothing is kept
+    if (none) {
         const size_t elem = dtype == CLB_F64 ? 8 : dtype == CLB_F32 ? 4 : 2;
         e = cudaMemset2DAsync(y, (size_t)(rows > 1 ? ldy : cols) * elem, 0, (size_t)cols * elem, (size_t)rows, s);
         return e == cudaSuccess ? CLB_OK : set_error(CLB_ERR_CUDA, cudaGetErrorString(e));

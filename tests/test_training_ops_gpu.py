@@ -138,6 +138,20 @@ def test_dropout_rates(p, rescale):
         assert torch.equal(y == 0, want == 0)
 
 
+def test_dropout_rates_that_round_to_one_keep_nothing():
+    """p 2^32 rounds to 2^32, which no word reaches, not even the largest."""
+    for seed, offset, i, j in [(11, 1686893, 18, 48), (11, 3385604, 33, 13)]:
+        assert int(words(64, 64, seed, offset)[i, j]) == 0xFFFFFFFF
+        for dtype in ALL:
+            for layout in LAYOUTS:
+                x = laid(torch.ones(64, 64, device="cuda", dtype=dtype), layout)
+                for p in (1.0, 1 - 2.0 ** -34, 1 - 2.0 ** -33, 1 - 2.0 ** -50):  # round(p 2^32) goes to the even one
+                    assert not cl.dropout(x, p, seed=seed, offset=offset).any()
+                for p in (1 - 2.0 ** -32, 0.5):
+                    y = cl.dropout(x, p, seed=seed, offset=offset, rescale=False)
+                    assert torch.equal(y, dropped(x, p, seed, offset, False)) and y[i, j] == 1
+
+
 def test_dropout_shapes_and_refusals():
     for shape in [(0, 5), (5, 0), (7,), (), (3, 4, 5), (2, 3, 4, 5)]:
         x = rand(shape, 4)
