@@ -119,18 +119,22 @@ def _dropout(x, p, rescale, seed, offset, rng):
     if not 0.0 <= p <= 1.0:
         raise ValueError(f"dropout: p must be in [0, 1], got {p}")
     _check("dropout", x)
-    grad = x.requires_grad and torch.is_grad_enabled()
-    if x.dim() == 2:
-        if not grad:
-            return _drop(x, p, rescale, seed, offset, rng)
-        # between logic layers with 16-bit activations the gradient is handed over in fp32, past autograd's rounding
-        out_slot = GradSlot() if x.dtype in _LOW else None
-        y = _DropoutFn.apply(x, p, rescale, seed, offset, rng, getattr(x, "_clb_slot", None), out_slot)
-        if out_slot is not None:
-            y._clb_slot = out_slot
-        return y
-    flat = x.reshape(x.shape[0], -1) if x.dim() > 2 and x.shape[0] else x.reshape(1, -1)
-    return _DropoutFn.apply(flat, p, rescale, seed, offset, rng, None, None).reshape(x.shape)
+    flat = x if x.dim() == 2 else x.reshape(x.shape[0], -1) if x.dim() > 2 and x.shape[0] else x.reshape(1, -1)
+    out_slot = None
+    if x.requires_grad and torch.is_grad_enabled():
+        # between logic layers (conv layers' outputs have four axes) with 16-bit activations the gradient is handed over in
+        # fp32, past autograd's rounding
+        in_slot = None
+        if x.dim() > 1 and x.dtype in _LOW:
+            in_slot, out_slot = getattr(x, "_clb_slot", None), GradSlot()
+        y = _DropoutFn.apply(flat, p, rescale, seed, offset, rng, in_slot, out_slot)
+    else:
+        y = _drop(flat, p, rescale, seed, offset, rng)
+    if x.dim() != 2:
+        y = y.reshape(x.shape)
+    if out_slot is not None:
+        y._clb_slot = out_slot
+    return y
 
 
 def dropout(x: torch.Tensor, p: float = 0.5, *, seed: int, offset: int = 0, rescale: bool = True) -> torch.Tensor:

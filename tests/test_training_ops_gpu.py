@@ -311,6 +311,44 @@ def test_dropout_between_logic_layers(dtype):
         assert (g - w).abs().max() <= tol * w.abs().max()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_dropout_between_conv_layers(dtype):
+    """As between dense layers: with 16-bit activations the gradient passes in fp32."""
+    torch.manual_seed(0)
+    a = cl.ConvLayer((3, 8, 8), 1, 8, 3, 2, num_gates=4).cuda()
+    b = cl.ConvLayer((8, 4, 4), 1, 16, 3, 2, num_gates=4).cuda()
+    x = torch.rand(20, 3, 8, 8, device="cuda").to(dtype)
+    drop = lambda h: cl.dropout(h, 0.25, seed=3, rescale=False)  # noqa: E731
+    h = drop(a(x))
+    assert h.shape == (20, 8, 4, 4)
+    y = b(h)
+    gy = rand(y.shape, 6, dtype)
+    got = torch.autograd.grad(y, [a.weights, b.weights], gy)
+    h = a(x)
+    mask = dropped(torch.ones(20, 128, device="cuda", dtype=dtype), 0.25, 3, 0, False).reshape(h.shape)
+    mid = (h.detach() * mask).requires_grad_()
+    if dtype == torch.float32:
+        y2 = b(mid)
+        gmid, gwb = torch.autograd.grad(y2, [mid, b.weights], gy)
+        gwa, = torch.autograd.grad(h, a.weights, gmid * mask)
+    else:
+        from compactlogic_b200.functional import GradSlot
+        mid._clb_slot = GradSlot()
+        y2 = b(mid)
+        gwb, _ = torch.autograd.grad(y2, [b.weights, mid], gy)
+        h._clb_slot.add(mid._clb_slot.grad * mask.reshape(20, -1).t().float())
+        gwa, = torch.autograd.grad(h, a.weights, torch.zeros((), dtype=dtype, device="cuda").expand(h.shape))
+    assert torch.equal(y, y2)
+    for g, w in zip(got, (gwa, gwb)):
+        assert (g - w).abs().max() <= 1e-5 * w.abs().max()
+    # another consumer beside the layer: its share comes through autograd
+    h = drop(a(x))
+    both, = torch.autograd.grad([b(h), h], a.weights, [gy, torch.ones_like(h)])
+    h = drop(a(x))
+    alone, = torch.autograd.grad(h, a.weights, torch.ones_like(h))
+    assert (both - (got[0] + alone)).abs().max() <= 1e-5 * both.abs().max()
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("reentrant", [True, False])
 def test_logic_layers_and_dropout_recomputed(reentrant, dtype):
