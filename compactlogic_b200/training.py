@@ -28,21 +28,10 @@ _ACC = {torch.float32: torch.float32, torch.bfloat16: torch.float32, torch.float
 _BYTES = {torch.float32: 4, torch.float64: 8}
 
 # The small calls of a training step are bound by the host, so the paths below keep to one allocation where several buffers
-# live and die together, and look up the current stream by its device index.
+# live and die together, and look up the current stream by its device index.  A launch goes to the current GPU: where a public
+# call's input is on another one, the call starts over with that one current (autograd's backward passes have it so).
 _stream = torch._C._cuda_getCurrentRawStream
 _device = torch._C._cuda_getDevice
-
-
-def _run(name: str, x: torch.Tensor, *args) -> None:
-    """One entry point, on the GPU of ``x`` (also where another is the current one) and the current stream there."""
-    index = x.get_device()
-    if index == _device():
-        status = getattr(L.lib(), name)(*args, _stream(index))
-    else:
-        with torch.cuda.device(index):
-            status = getattr(L.lib(), name)(*args, _stream(index))
-    if status:
-        L.check(status, name)
 
 
 # ------------------------------------------------------------------------------------------------------------ layouts
@@ -88,8 +77,10 @@ def _drop(x: torch.Tensor, p: float, rescale: bool, seed: int, offset: int, rng:
     n, d = x.shape
     if inner:
         n, d = d, n
-    _run("clb_dropout", x, L.dtype_code(x.dtype), x.data_ptr(), ld, n, d, inner, p, rescale, seed, offset,
-         rng.data_ptr() if rng is not None else 0, y.data_ptr(), d)
+    status = L.lib().clb_dropout(L.dtype_code(x.dtype), x.data_ptr(), ld, n, d, inner, p, rescale, seed, offset,
+                                 rng.data_ptr() if rng is not None else 0, y.data_ptr(), d, _stream(x.get_device()))
+    if status:
+        L.check(status, "clb_dropout")
     return y
 
 
@@ -119,6 +110,9 @@ def _dropout(x, p, rescale, seed, offset, rng):
     if not 0.0 <= p <= 1.0:
         raise ValueError(f"dropout: p must be in [0, 1], got {p}")
     _check("dropout", x)
+    if x.get_device() != _device():
+        with torch.cuda.device(x.device):
+            return _dropout(x, p, rescale, seed, offset, rng)
     flat = x if x.dim() == 2 else x.reshape(x.shape[0], -1) if x.dim() > 2 and x.shape[0] else x.reshape(1, -1)
     out_slot = None
     if x.requires_grad and torch.is_grad_enabled():
@@ -141,10 +135,10 @@ def dropout(x: torch.Tensor, p: float = 0.5, *, seed: int, offset: int = 0, resc
     """Zero each entry of ``x`` with probability ``p`` (in steps of 2^-32) and scale the others by 1 / (1 - p), or leave them
     as they are with ``rescale=False`` (soft bits then stay in [0, 1]).
 
-    Entry (i, j) of ``x`` taken as [first axis, all others] is kept when its word of Philox4x32-10 under the key ``seed``
-    and the counter (j / 2, i / 2, ``offset``) is at least p 2^32: the mask depends on seed, offset and place alone, not
-    on layout, strides or type, and is not stored.  Use another ``offset`` for each pass.  A dropped entry is 0 whatever it
-    held."""
+    Entry (i, j) of ``x`` taken as [first axis, all others] (a tensor of one axis as a single row [1, all]) is kept when its
+    word of Philox4x32-10 under the key ``seed`` and the counter (j / 2, i / 2, ``offset``) is at least p 2^32, rounded: the
+    mask depends on seed, offset and place alone, not on layout, strides or type, and is not stored.  Use another ``offset``
+    for each pass.  A dropped entry is 0 whatever it held."""
     if not (0 <= seed < 1 << 64 and 0 <= offset < 1 << 64):
         raise ValueError("dropout: seed and offset are unsigned 64-bit numbers")
     return _dropout(x, p, rescale, seed, offset, None)
@@ -165,7 +159,9 @@ class LogicDropout(torch.nn.Module):
 
     The buffer ``rng_state`` (int64 {seed, offset}) advances on the device, so a captured training step
     (``compactlogic_b200.graph``) draws a new mask at each replay, and a loaded checkpoint continues the sequence.  ``seed``
-    defaults to a draw from torch's generator.  Passes of one module on several streams at once are not ordered.
+    defaults to a draw from torch's generator.  Passes of one module on several streams at once are not ordered.  Data-parallel
+    ranks with equal states mask their samples alike: after buffers were broadcast or loaded, give each rank a seed of its own
+    (``m.rng_state[0] += rank``).
 
     A pass that activation checkpointing (``torch.utils.checkpoint``, either form) computes again draws the mask of the pass
     that it repeats.  The two are matched by where torch's CUDA generator stands, which checkpointing puts back
@@ -212,7 +208,9 @@ class LogicDropout(torch.nn.Module):
                                    "generator alike for two passes in flight")
             return used
         used = torch.empty(2, dtype=torch.int64, device=x.device)
-        _run("clb_dropout_advance", x, self.rng_state.data_ptr(), used.data_ptr())
+        status = L.lib().clb_dropout_advance(self.rng_state.data_ptr(), used.data_ptr(), _stream(x.get_device()))
+        if status:
+            L.check(status, "clb_dropout_advance")
         if place is not None:
             used.shared_place = place in self._passes
             self._passes[place] = used
@@ -225,6 +223,9 @@ class LogicDropout(torch.nn.Module):
             return x
         _check("LogicDropout", x)
         _same_device("LogicDropout", x, "rng_state", self.rng_state)
+        if x.get_device() != _device():
+            with torch.cuda.device(x.device):
+                return self.forward(x)
         return _dropout(x, self.p, self.rescale, 0, 0, self._draw(x))
 
     def extra_repr(self):
@@ -252,8 +253,11 @@ def _norm_forward(x, weight, bias, eps, keep):
     stats = torch.empty(2 * n, dtype=acc, device=x.device) if keep else None
     at = stats.data_ptr() if keep else 0
     nbytes, ws = _norm_workspace(code, n, d, inner, 0, x.device)
-    _run("clb_layer_norm_forward", x, code, x.data_ptr(), ld, n, d, inner, L.ptr(weight), L.ptr(bias), eps, y.data_ptr(),
-         n if inner else d, at, at + n * _BYTES[acc] if keep else 0, L.ptr(ws), nbytes)
+    status = L.lib().clb_layer_norm_forward(code, x.data_ptr(), ld, n, d, inner, L.ptr(weight), L.ptr(bias), eps,
+                                            y.data_ptr(), n if inner else d, at, at + n * _BYTES[acc] if keep else 0,
+                                            L.ptr(ws), nbytes, _stream(x.get_device()))
+    if status:
+        L.check(status, "clb_layer_norm_forward")
     return y, x, stats
 
 
@@ -281,10 +285,15 @@ class _LayerNormFn(torch.autograd.Function):
         code = L.dtype_code(x.dtype)
         nbytes, ws = _norm_workspace(code, n, d, inner, 1, x.device)
         at = stats.data_ptr()
-        _run("clb_layer_norm_backward", x, code, x.data_ptr(), ld, gy.data_ptr(), ldg, n, d, inner, L.ptr(weight), at,
-             at + n * _BYTES[acc], L.ptr(gx), n if inner else d, L.ptr(gw), L.ptr(gb), L.ptr(ws), nbytes)
-        return (first_order("layer_norm", gx, x, weight, given), first_order("layer_norm", gw, x, given),
-                first_order("layer_norm", gb, given), None)
+        status = L.lib().clb_layer_norm_backward(code, x.data_ptr(), ld, gy.data_ptr(), ldg, n, d, inner, L.ptr(weight), at,
+                                                 at + n * _BYTES[acc], L.ptr(gx), n if inner else d, L.ptr(gw), L.ptr(gb),
+                                                 L.ptr(ws), nbytes, _stream(x.get_device()))
+        if status:
+            L.check(status, "clb_layer_norm_backward")
+        if torch.is_grad_enabled():
+            gx, gw, gb = (first_order("layer_norm", gx, x, weight, given), first_order("layer_norm", gw, x, given),
+                          first_order("layer_norm", gb, given))
+        return gx, gw, gb, None
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
@@ -294,6 +303,9 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     ``weight`` and ``bias`` (optional, [features]) are fp32 for fp32, bf16 and fp16 activations and fp64 for fp64, as the
     layers' parameters are; statistics and the parameters' gradients are summed in that type, in a fixed order."""
     _check("layer_norm", x)
+    if x.get_device() != _device():
+        with torch.cuda.device(x.device):
+            return layer_norm(x, weight, bias, eps)
     if x.dim() < 1 or x.shape[-1] < 1:
         raise RuntimeError(f"layer_norm: expected [..., features], got shape {tuple(x.shape)}")
     acc = _ACC[x.dtype]
@@ -379,8 +391,11 @@ def _logit_grad(z, actions, mask, temperature, stats, slope, scale, upstream, up
     fresh = gz is None
     if fresh:
         gz = _like(z, inner)
-    _run("clb_logit_grad", z, L.dtype_code(z.dtype), z.data_ptr(), ld, n, v, inner, actions.data_ptr(), L.ptr(mask),
-         temperature, stats, slope, scale, upstream.data_ptr(), up_stride, not fresh, gz.data_ptr(), n if inner else v)
+    status = L.lib().clb_logit_grad(L.dtype_code(z.dtype), z.data_ptr(), ld, n, v, inner, actions.data_ptr(), L.ptr(mask),
+                                    temperature, stats, slope, scale, upstream.data_ptr(), up_stride, not fresh,
+                                    gz.data_ptr(), n if inner else v, _stream(z.get_device()))
+    if status:
+        L.check(status, "clb_logit_grad")
     return gz
 
 
@@ -390,8 +405,10 @@ def _logp_forward(z, actions, mask, temperature, keep):
     acc = _ACC[z.dtype]
     logp = torch.empty(n, dtype=acc, device=z.device)
     stats = torch.empty(2 * n, dtype=acc, device=z.device) if keep else None
-    _run("clb_action_logp", z, L.dtype_code(z.dtype), z.data_ptr(), ld, n, v, inner, actions.data_ptr(), L.ptr(mask),
-         temperature, logp.data_ptr(), L.ptr(stats))
+    status = L.lib().clb_action_logp(L.dtype_code(z.dtype), z.data_ptr(), ld, n, v, inner, actions.data_ptr(), L.ptr(mask),
+                                     temperature, logp.data_ptr(), L.ptr(stats), _stream(z.get_device()))
+    if status:
+        L.check(status, "clb_action_logp")
     return logp, z, stats
 
 
@@ -424,6 +441,9 @@ def action_log_probs(logits: torch.Tensor, actions: torch.Tensor, *, mask: Optio
     Rows where ``mask`` (bool [...]) is False are not read: their value and gradient are 0 and their action may be
     anything.  In other rows an action outside [0, classes) gives NaN."""
     z, act, m, lead = _rows_of("action_log_probs", logits, actions, mask)
+    if z.get_device() != _device():
+        with torch.cuda.device(z.device):
+            return action_log_probs(logits, actions, mask=mask, temperature=temperature)
     _check_temperature("action_log_probs", temperature)
     if z.requires_grad and torch.is_grad_enabled():
         logp = _LogProbFn.apply(_dense(z), act, m, temperature)
@@ -456,11 +476,13 @@ def _policy(z, actions, mask, adv, old, ref, low, high, kl_coef, temperature, re
     at, size = kept.data_ptr(), _BYTES[acc]
     # the mean's and the sum's gradient is made in the same pass, for an upstream gradient of 1
     gz = _like(z, inner) if grad and not per_row else None
-    _run("clb_policy_loss", z, L.dtype_code(z.dtype), z.data_ptr(), ld, n, v, inner, actions.data_ptr(), L.ptr(mask),
-         adv.data_ptr(), old.data_ptr(), L.ptr(ref), low, high, kl_coef, temperature, reduction == "mean",
-         0 if per_row else loss.data_ptr(), at + 3 * n * size, loss.data_ptr() if per_row else at + (3 * n + 1) * size,
-         logp.data_ptr(), ratio.data_ptr(), L.ptr(kl), at if grad else 0, at + n * size if grad else 0, L.ptr(gz),
-         n if inner else v)
+    status = L.lib().clb_policy_loss(
+        L.dtype_code(z.dtype), z.data_ptr(), ld, n, v, inner, actions.data_ptr(), L.ptr(mask), adv.data_ptr(), old.data_ptr(),
+        L.ptr(ref), low, high, kl_coef, temperature, reduction == "mean", 0 if per_row else loss.data_ptr(),
+        at + 3 * n * size, loss.data_ptr() if per_row else at + (3 * n + 1) * size, logp.data_ptr(), ratio.data_ptr(),
+        L.ptr(kl), at if grad else 0, at + n * size if grad else 0, L.ptr(gz), n if inner else v, _stream(z.get_device()))
+    if status:
+        L.check(status, "clb_policy_loss")
     return loss, logp, ratio, kl, z, gz, kept
 
 
@@ -506,8 +528,13 @@ def policy_loss(logits: torch.Tensor, actions: torch.Tensor, advantages: torch.T
     are not read, give zeros, and get a zero gradient; a counted row whose action is outside [0, classes) gives NaN.
 
     With "mean" and "sum" the logit gradient is computed in the forward pass, for an upstream gradient of 1; ``backward``
-    hands it over, or computes it anew where the upstream gradient is another (a scaled loss)."""
+    hands it over, or computes it anew where the upstream gradient is another (a scaled loss).  Between the two passes the
+    call holds that gradient, as large as the logits, outside the saved tensors that offloading hooks see."""
     z, act, m, lead = _rows_of("policy_loss", logits, actions, mask)
+    if z.get_device() != _device():
+        with torch.cuda.device(z.device):
+            return policy_loss(logits, actions, advantages, old_log_probs, ref_log_probs=ref_log_probs, mask=mask, clip=clip,
+                               kl_coef=kl_coef, temperature=temperature, reduction=reduction)
     _check_temperature("policy_loss", temperature)
     if reduction not in ("mean", "sum", "none"):
         raise ValueError(f"policy_loss: reduction must be mean, sum or none, got {reduction!r}")

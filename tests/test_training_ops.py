@@ -80,40 +80,62 @@ def test_c_entry_points_refuse_without_a_gpu():
         assert lib.clb_logit_grad(*a) == status, (at, value)
 
 
-def test_entry_points_run_on_their_inputs_gpu(monkeypatch):
-    """Where another GPU is the current one, the input's is made current around the call, and its stream is taken."""
+def test_public_calls_start_over_on_their_inputs_gpu(monkeypatch):
+    """Where another GPU is the current one, the input's is made current around the whole call: for a stand-in of a tensor of
+    GPU 1, the launch comes with that one current, and the other is current again afterwards."""
     from compactlogic_b200 import training as T
-    calls, entered = [], []
+    log = []
 
     class On:
-        def __init__(self, index):
-            self.index = index
+        def __init__(self, device):
+            self.index = device.index
 
         def __enter__(self):
-            entered.append(self.index)
+            log.append(("enter", self.index))
+            self.before, state.current = state.current, self.index
 
         def __exit__(self, *error):
-            entered.append(None)
+            state.current = self.before
 
-    class Lib:
-        def clb_probe(self, *args):
-            calls.append((args, list(entered)))
-            return self.status
+    class Far(torch.Tensor):  # on the CPU, says that it is on GPU 1
+        is_cuda = True
+        device = torch.device("cuda", 1)
 
-    class Input:
+        @classmethod
+        def __torch_function__(cls, func, types, args=(), kwargs=None):
+            with torch._C.DisableTorchFunctionSubclass():
+                out = func(*args, **(kwargs or {}))
+            return out.as_subclass(Far) if isinstance(out, torch.Tensor) else out
+
         def get_device(self):
             return 1
 
-    fake = Lib()
-    fake.status = L.CLB_OK
-    monkeypatch.setattr(T, "_stream", lambda index: 100 + index)
+    class state:
+        current = 0
+
+    class Launched(Exception):
+        pass
+
+    def launch(*args):
+        log.append(("launch", state.current))
+        raise Launched
+
+    monkeypatch.setattr(T, "_device", lambda: state.current)
     monkeypatch.setattr(T.torch.cuda, "device", On)
-    monkeypatch.setattr(T.L, "lib", lambda: fake)
-    for current in (0, 1):
-        monkeypatch.setattr(T, "_device", lambda: current)
-        T._run("clb_probe", Input(), 7, 8)
-    assert calls == [((7, 8, 101), [1]), ((7, 8, 101), [1, None])] and entered == [1, None]
-    fake.status = L.CLB_ERR_INVALID
-    fake.clb_last_error = lambda: b"no"
-    with pytest.raises(RuntimeError, match="clb_probe"):
-        T._run("clb_probe", Input())
+    for name in ("_drop", "_norm_forward", "_logp_forward", "_policy"):
+        monkeypatch.setattr(T, name, launch)
+    x, one = torch.zeros(4, 8).as_subclass(Far), torch.zeros(4).as_subclass(Far)
+    act = torch.zeros(4, dtype=torch.int64).as_subclass(Far)
+    m = cl.LogicDropout(0.5)
+    m.rng_state = m.rng_state.as_subclass(Far)
+    monkeypatch.setattr(m, "_draw", lambda t: log.append(("draw", state.current)))
+    for call in (lambda: cl.dropout(x, 0.5, seed=1), lambda: cl.layer_norm(x), lambda: cl.action_log_probs(x, act),
+                 lambda: cl.policy_loss(x, act, one, one), lambda: m(x)):
+        for current in (0, 1):
+            state.current = current
+            log.clear()
+            with pytest.raises(Launched):
+                call()
+            assert log[-1] == ("launch", 1) and state.current == current
+            assert [e for e in log if e[0] == "enter"] == ([] if current else [("enter", 1)])
+            assert all(at == 1 for what, at in log if what == "draw")
