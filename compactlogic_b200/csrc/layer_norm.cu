@@ -8,10 +8,12 @@
 // Forms: rows contiguous, up to 8 blocks of a cluster a row (norm_line_*); samples contiguous (norm_strip_*); wider rows and
 // fp64 (norm_rows_*, norm_cols_*, norm_weight_*), which read their operands up to three times.
 // Measured on a B200 (6.45 TB/s copy rate): bf16 8192 x 4096, forward 37 us (134 MB) and backward 55 us (201 MB and the
-// weight's gradients); fp32 8192 x 4096 forward 56 us (268 MB, 75 %); fp32 16384 features x 512 samples, samples contiguous,
-// both passes 56 us (168 MB at least).  What bounds the rows is the issue of some 15 instructions an entry (forward) and 29
-// (backward) and two block barriers a row; what bounds the strips is that each pass reads its operands twice, and six
-// launches.
+// weight's gradients); fp32 8192 x 4096 forward 55 us (268 MB, 75 %); fp32 16384 features x 512 samples, samples contiguous,
+// both passes 56 us (168 MB at least).  What bounds the 16-bit rows is waiting: 15 instructions an entry fill 44 % of the issue
+// slots and 30 % of the DRAM's rate in the forward pass, 31 an entry 62 % and 40 % in the backward pass, while 16 warps an SM
+// wait for shared memory, for weight and bias, and for one another at two barriers a row.  What bounds the strips is that each
+// pass reads its operands twice, and six launches.  Rows wider than the forward plan (40960 fp32, 81920 16-bit entries) are
+// read three times: fp32 1024 x 65536 forward 406 us (537 MB).
 #include <cuda_runtime.h>
 
 #include <atomic>
@@ -339,8 +341,10 @@ __device__ __forceinline__ void parameter(const float* __restrict__ v, int c, in
 constexpr int kMostParts = 8;  // blocks of a row
 
 // Threads of a block; the forward kernel has two blocks an SM, the gradient kernel one.  More threads leave each fewer
-// registers: bf16 8192 x 4096 forward takes 29.7 us with 320, 32.8 with 384, 35.4 with 512 (which spills); forward and
-// gradients 96 with 640 threads of two windows, 103 with 512 of four; wider rows need four.
+// registers (512 in the forward kernel spill).  Forward pass with 320, 384 and 512: fp16 3001 x 5001 28.8, 29.9 and 32.2 us, but
+// bf16 8192 x 4096 37.0, 31.4 and 34.2, fp32 8192 x 4096 56.4, 51.8 and 49.4.  Forward and gradients of bf16 8192 x 4096: 96 us
+// with gradient blocks of 640 threads of two windows, 103 with 512 of four (before the parameters were read in 32 bytes); wider
+// rows need four.
 constexpr int kLineThreads = 320;
 template <int NP> constexpr int kGradThreads = NP <= 2 ? 640 : 512;
 
@@ -752,7 +756,8 @@ unsigned blocks(int64_t n) { return (unsigned)(n < (1 << 30) ? n : (1 << 30)); }
 // strip of 32 V samples (V a 16-byte pack, or 1 where rows do not start on 16 bytes) and walks down features 8 at a time,
 // all 8 loads in flight; the blocks of `chunk` features leave partial results, which a small kernel folds.  Second pass:
 // elementwise, reading the operands again, out of the L2 cache where they fit.  (Running both passes over one slab of samples
-// after the other, each small enough to stay there, was slower: fp32 64000 x 1024 forward 267 us, in one go 156.)
+// after the other, each small enough to stay there, was slower: fp32 64000 x 1024 forward 267 us, in one go
+// 156, and 139 since three blocks an SM are resident.)
 
 constexpr int kColThreads = 256, kBatch = 8;
 

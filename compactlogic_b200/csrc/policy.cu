@@ -19,7 +19,7 @@
 // Measured on a B200 (6.45 TB/s copy rate): bf16 2048 x 131072 with its gradient 242 us (1.07 GB, 4.4 TB/s, 69 %), fp32 1777 x
 // 50001 with a third of the rows masked 147 us (63 %), log-probabilities of bf16 4096 x 32768 with their gradient 135 us (805
 // MB over the two calls, 93 %).  What bounds the long rows: two exponentials an entry (16 a clock and SM: 119 of the 242 us)
-// among 12 instructions, and the wait of a cluster's blocks for one another between the two halves.  Measured and dropped:
+// among 14 instructions, and the wait of a cluster's blocks for one another between the two halves.  Measured and dropped:
 // clusters that walk over the rows with the next row on its way to shared memory (308 us: fewer clusters fit than blocks),
 // and one block a row that reads the row again out of the L2 cache (242 to 276 us).
 #include <cuda_runtime.h>
